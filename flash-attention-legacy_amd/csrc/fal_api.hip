@@ -807,3 +807,215 @@ int fal_decode_noalloc(const void* q, const void* k_cache, const void* v_cache, 
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Paged KV cache
+// ---------------------------------------------------------------------------
+namespace {
+
+// A cache operand: rows (page, head, row) of head_dim elements of `bytes` each.
+int check_cache(const char* name, const fal_paged_cache& c, const void* p, const int64_t* st, bool written) {
+  const int64_t bytes = c.fp8 ? 1 : 2;
+  if (!p && c.num_pages > 0) return fail(FAL_ERR_INVALID, "%s: null pointer", name);
+  if (!aligned16(p)) return fail(FAL_ERR_INVALID, "%s: base pointer must be 16-byte aligned", name);
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] * bytes % 16 != 0)
+      return fail(FAL_ERR_INVALID, "%s: stride[%d]=%lld must be a non-negative multiple of 16 bytes", name, i,
+                  (long long)st[i]);
+  // kernels address the rows of a page with 32-bit byte offsets
+  if (st[2] >= (int64_t(1) << 22))
+    return fail(FAL_ERR_UNSUPPORTED, "%s: row stride %lld elements is too large (limit 4194304)", name,
+                (long long)st[2]);
+  if (st[2] < c.head_dim)
+    return fail(FAL_ERR_UNSUPPORTED, "%s: row stride %lld is shorter than a row of %lld elements", name,
+                (long long)st[2], (long long)c.head_dim);
+  if (!written) return FAL_OK;
+  // no two rows of a cache that is written may share memory: in the order of their strides,
+  // each axis steps over all that the ones before it span
+  struct Axis { int64_t stride, size; } ax[3] = {{st[0], c.num_pages}, {st[1], c.heads_kv}, {st[2], c.page_size}};
+  std::sort(ax, ax + 3, [](const Axis& a, const Axis& b) { return a.stride < b.stride; });
+  int64_t span = c.head_dim;
+  for (const Axis& a : ax) {
+    if (a.size <= 1) continue;
+    if (a.stride < span)
+      return fail(FAL_ERR_INVALID, "%s: rows overlap (stride %lld over %lld elements)", name, (long long)a.stride,
+                  (long long)span);
+    if (a.stride > (int64_t(1) << 61) / a.size) return fail(FAL_ERR_INVALID, "%s: stride too large", name);
+    span += a.stride * (a.size - 1);
+  }
+  return FAL_OK;
+}
+
+int check_scale(const char* name, const fal_paged_cache& c, const float* p, const int64_t* st, bool written) {
+  if (!c.fp8) return p ? fail(FAL_ERR_INVALID, "%s: a 16-bit cache has no scales", name) : FAL_OK;
+  if (!p && c.num_pages > 0) return fail(FAL_ERR_INVALID, "%s: null pointer", name);
+  if (reinterpret_cast<uintptr_t>(p) & 3) return fail(FAL_ERR_INVALID, "%s: base pointer must be 4-byte aligned", name);
+  if (st[0] < 0 || st[1] < 0) return fail(FAL_ERR_INVALID, "%s: negative stride", name);
+  if (!written) return FAL_OK;
+  const bool by_page = st[0] >= st[1];   // which axis is the outer one
+  const int64_t inner = by_page ? st[1] : st[0], outer = by_page ? st[0] : st[1];
+  const int64_t n_in = by_page ? c.heads_kv : c.num_pages, n_out = by_page ? c.num_pages : c.heads_kv;
+  if ((n_in > 1 && inner < 1) || (n_out > 1 && (outer < 1 || outer / std::max<int64_t>(inner, 1) < n_in)))
+    return fail(FAL_ERR_INVALID, "%s: entries overlap", name);
+  return FAL_OK;
+}
+
+// What both calls share: sizes, page table, token ranges and caches.
+int fill_paged(PagedCache& p, const fal_paged_cache* cache, int bf16, bool written) {
+  if (!cache) return fail(FAL_ERR_INVALID, "cache: null pointer");
+  const fal_paged_cache& c = *cache;
+  if (!head_dim_ok(c.head_dim))
+    return fail(FAL_ERR_UNSUPPORTED, "head_dim must be 32, 64, 96, 128, or 256, got %lld", (long long)c.head_dim);
+  if (!dims_ok(c.batch) || !dims_ok(c.seqlen) || !dims_ok(c.total_tokens) || !dims_ok(c.num_pages) ||
+      c.heads_q <= 0 || c.heads_kv <= 0 || c.heads_q > 0xffff)
+    return fail(FAL_ERR_INVALID, "invalid sizes");
+  if (c.heads_q % c.heads_kv != 0)
+    return fail(FAL_ERR_INVALID, "num_heads_q (%lld) must be divisible by num_heads_kv (%lld)", (long long)c.heads_q,
+                (long long)c.heads_kv);
+  if (c.page_size <= 0 || c.page_size % 16 != 0 || c.page_size > (1 << 16))
+    return fail(FAL_ERR_UNSUPPORTED, "page_size must be a multiple of 16 up to 65536, got %lld", (long long)c.page_size);
+  if (c.max_pages < 0 || c.max_pages > 0x7fffffff / c.page_size)
+    return fail(FAL_ERR_INVALID, "page_table: max_pages * page_size must stay below 2^31");
+  if (!c.cu_seqlens && c.total_tokens != c.batch * c.seqlen)
+    return fail(FAL_ERR_INVALID, "total_tokens must be batch * seqlen");
+  if (c.batch == 0 && c.total_tokens > 0) return fail(FAL_ERR_INVALID, "tokens without a sequence");
+  if (c.batch > 0 && !c.cache_seqlens) return fail(FAL_ERR_INVALID, "cache_seqlens: null pointer");
+  if (c.batch > 0 && c.max_pages > 0 && !c.page_table) return fail(FAL_ERR_INVALID, "page_table: null pointer");
+  if (c.table_stride < 0) return fail(FAL_ERR_INVALID, "page_table: negative stride");
+  int rc;
+  if ((rc = check_cache("k_cache", c, c.k, c.k_strides, written)) ||
+      (rc = check_cache("v_cache", c, c.v, c.v_strides, written)) ||
+      (rc = check_scale("k_scale", c, c.k_scale, c.k_scale_strides, written)) ||
+      (rc = check_scale("v_scale", c, c.v_scale, c.v_scale_strides, written)))
+    return rc;
+  p.k = c.k, p.v = c.v, p.k_scale = c.k_scale, p.v_scale = c.v_scale;
+  p.table = c.page_table, p.table_sb = c.table_stride;
+  p.seqlens = c.cache_seqlens, p.cu = c.cu_seqlens;
+  p.k_sp = c.k_strides[0], p.k_sh = c.k_strides[1], p.k_ss = c.k_strides[2];
+  p.v_sp = c.v_strides[0], p.v_sh = c.v_strides[1], p.v_ss = c.v_strides[2];
+  p.ks_sp = c.k_scale_strides[0], p.ks_sh = c.k_scale_strides[1];
+  p.vs_sp = c.v_scale_strides[0], p.vs_sh = c.v_scale_strides[1];
+  p.B = (int)c.batch, p.n = (int)c.seqlen, p.total = (int)c.total_tokens;
+  p.Hq = (int)c.heads_q, p.Hkv = (int)c.heads_kv;
+  p.num_pages = (int)c.num_pages, p.page_size = (int)c.page_size, p.capacity = (int)(c.max_pages * c.page_size);
+  p.fp8 = c.fp8 != 0, p.bf16 = bf16;
+  return FAL_OK;
+}
+
+// A 16-bit tensor of tokens, addressed row by row.
+int check_tokens(const char* name, const void* p, const int64_t* st, bool batched) {
+  if (!p) return fail(FAL_ERR_INVALID, "%s: null pointer", name);
+  if (!st) return fail(FAL_ERR_INVALID, "%s: null strides", name);
+  if (!aligned16(p)) return fail(FAL_ERR_INVALID, "%s: base pointer must be 16-byte aligned", name);
+  for (int i = batched ? 0 : 1; i < 3; ++i)
+    if (st[i] % 8 != 0 || st[i] < 0)
+      return fail(FAL_ERR_INVALID, "%s: stride[%d]=%lld must be a non-negative multiple of 8", name, i,
+                  (long long)st[i]);
+  return FAL_OK;
+}
+
+int paged_append_impl(const fal_paged_cache* cache, const void* k, const void* v, const void* q, void* q_out,
+                      const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+                      const int64_t* q_out_strides, const float* rotary_cos, const float* rotary_sin,
+                      int64_t rotary_rows, int64_t cos_stride, int64_t sin_stride, int64_t rotary_dim,
+                      int rotary_interleaved, void* stream, int bf16) {
+  PagedAppendParams p{};
+  int rc = fill_paged(p.c, cache, bf16, true);
+  if (rc) return rc;
+  const fal_paged_cache& c = *cache;
+  if (rotary_dim < 0 || rotary_dim > c.head_dim || rotary_dim % 16 != 0)
+    return fail(FAL_ERR_UNSUPPORTED, "rotary_dim must be a multiple of 16 up to head_dim, got %lld", (long long)rotary_dim);
+  if (rotary_dim > 0) {
+    if (!rotary_cos || !rotary_sin) return fail(FAL_ERR_INVALID, "rotary tables: null pointer");
+    if (!aligned16(rotary_cos) || !aligned16(rotary_sin) || cos_stride % 4 != 0 || sin_stride % 4 != 0 ||
+        cos_stride < 0 || sin_stride < 0)
+      return fail(FAL_ERR_INVALID, "rotary tables: base pointers and rows must be 16-byte aligned");
+    if (rotary_rows < c.max_pages * c.page_size)
+      return fail(FAL_ERR_INVALID, "rotary tables: %lld rows for the %lld positions that the page table holds",
+                  (long long)rotary_rows, (long long)(c.max_pages * c.page_size));
+  }
+  if (c.total_tokens == 0) return ok();
+  const bool batched = !c.cu_seqlens;
+  if ((rc = check_tokens("k", k, k_strides, batched)) || (rc = check_tokens("v", v, v_strides, batched))) return rc;
+  if (q && ((rc = check_tokens("q", q, q_strides, batched)) || (rc = check_tokens("q_out", q_out, q_out_strides, batched))))
+    return rc;
+  p.k = k, p.v = v, p.q = q, p.q_out = q_out;
+  p.cos = rotary_cos, p.sin = rotary_sin;
+  p.cos_ss = cos_stride, p.sin_ss = sin_stride;
+  p.k_sb = k_strides[0], p.k_sh = k_strides[1], p.k_ss = k_strides[2];
+  p.v_sb = v_strides[0], p.v_sh = v_strides[1], p.v_ss = v_strides[2];
+  if (q) {
+    p.q_sb = q_strides[0], p.q_sh = q_strides[1], p.q_ss = q_strides[2];
+    p.qo_sb = q_out_strides[0], p.qo_sh = q_out_strides[1], p.qo_ss = q_out_strides[2];
+  }
+  p.rotary = (int)rotary_dim, p.interleaved = rotary_interleaved != 0;
+  // pages that seqlen rows can touch
+  p.pages_per_seq = (int)((std::max<int64_t>(c.seqlen, 1) + c.page_size - 2) / c.page_size + 1);
+  if (c.batch * p.pages_per_seq > 0x7fffffff / (2 * c.heads_kv) ||
+      c.batch * p.pages_per_seq * 2 * c.heads_kv + c.total_tokens * c.heads_q * c.head_dim / 16 / 64 >= 0x7fffffff)
+    return fail(FAL_ERR_INVALID, "problem too large for one launch");
+  return launch_status(launch_paged_append(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_append");
+}
+
+int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
+                    const int64_t* o_strides, float softmax_scale, int is_causal, void* workspace,
+                    size_t workspace_bytes, void* stream, int bf16) {
+  PagedAttnParams p{};
+  int rc = fill_paged(p.c, cache, bf16, false);
+  if (rc) return rc;
+  const fal_paged_cache& c = *cache;
+  if (c.total_tokens == 0) return ok();
+  const bool batched = !c.cu_seqlens;
+  if ((rc = check_tokens("q", q, q_strides, batched)) || (rc = check_tokens("o", o, o_strides, batched))) return rc;
+  const size_t need = fal_paged_attn_workspace_size(cache);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(FAL_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  p.q = q, p.o = o, p.lse = lse;
+  p.q_sb = q_strides[0], p.q_sh = q_strides[1], p.q_ss = q_strides[2];
+  p.o_sb = o_strides[0], p.o_sh = o_strides[1], p.o_ss = o_strides[2];
+  p.scale_log2 = scale_log2(softmax_scale);
+  p.negate_q = softmax_scale < 0.f;
+  p.causal = is_causal != 0;
+  if (c.total_tokens * c.heads_q > 0x7fffffff) return fail(FAL_ERR_INVALID, "problem too large for one launch");
+  return launch_status(launch_paged_attn(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_attn");
+}
+
+}  // namespace
+
+extern "C" {
+
+int fal_paged_append(const fal_paged_cache* cache, const void* k, const void* v, const void* q, void* q_out,
+                     const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+                     const int64_t* q_out_strides, const float* rotary_cos, const float* rotary_sin,
+                     int64_t rotary_rows, int64_t cos_stride, int64_t sin_stride, int64_t rotary_dim,
+                     int rotary_interleaved, void* stream) {
+  return paged_append_impl(cache, k, v, q, q_out, k_strides, v_strides, q_strides, q_out_strides, rotary_cos,
+                           rotary_sin, rotary_rows, cos_stride, sin_stride, rotary_dim, rotary_interleaved, stream, 0);
+}
+int fal_paged_append_bf16(const fal_paged_cache* cache, const void* k, const void* v, const void* q, void* q_out,
+                          const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+                          const int64_t* q_out_strides, const float* rotary_cos, const float* rotary_sin,
+                          int64_t rotary_rows, int64_t cos_stride, int64_t sin_stride, int64_t rotary_dim,
+                          int rotary_interleaved, void* stream) {
+  return paged_append_impl(cache, k, v, q, q_out, k_strides, v_strides, q_strides, q_out_strides, rotary_cos,
+                           rotary_sin, rotary_rows, cos_stride, sin_stride, rotary_dim, rotary_interleaved, stream, 1);
+}
+
+size_t fal_paged_attn_workspace_size(const fal_paged_cache* cache) {
+  (void)cache;
+  return 0;
+}
+int fal_paged_attn(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
+                   const int64_t* o_strides, float softmax_scale, int is_causal, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  return paged_attn_impl(cache, q, o, lse, q_strides, o_strides, softmax_scale, is_causal, workspace,
+                         workspace_bytes, stream, 0);
+}
+int fal_paged_attn_bf16(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
+                        const int64_t* o_strides, float softmax_scale, int is_causal, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  return paged_attn_impl(cache, q, o, lse, q_strides, o_strides, softmax_scale, is_causal, workspace,
+                         workspace_bytes, stream, 1);
+}
+
+}  // extern "C"

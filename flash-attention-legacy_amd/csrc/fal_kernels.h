@@ -135,6 +135,57 @@ struct DecodeParams {
   int bf16;           // element type of every fp16/bf16 tensor: 0 fp16, 1 bf16
 };
 
+// Paged KV cache: pages of `page_size` rows (a multiple of 16), `table` [B, max_pages] names the
+// page of every page_size rows of a sequence.  Element (page, row, head, e) of a cache lies at
+// page * c_sp + row * c_ss + head * c_sh + e.  fp8: codes are e4m3 and stand for code times the
+// page and head's scale.  Sequence b's tokens are rows cu[b]..cu[b + 1] of the packed tensors
+// or, without cu, rows 0..n of batch entry b.
+struct PagedCache {
+  void* k;
+  void* v;
+  float* k_scale;     // element (page, head) at page * ks_sp + head * ks_sh (fp8)
+  float* v_scale;
+  const int* table;
+  const int* seqlens; // [B] cache rows: before the new tokens (append), with them (attention)
+  const int* cu;      // [B + 1] packed tokens; null: n tokens in every sequence
+  int64_t k_sp, k_sh, k_ss;
+  int64_t v_sp, v_sh, v_ss;
+  int64_t ks_sp, ks_sh, vs_sp, vs_sh;
+  int64_t table_sb;
+  int B, n, Hq, Hkv;
+  int total;          // tokens in all (B * n without cu)
+  int num_pages, page_size, capacity;   // capacity = max_pages * page_size
+  int fp8;
+  int bf16;           // element type of the 16-bit tensors: 0 fp16, 1 bf16
+};
+
+// Rotation and append (fal_paged.hip).
+struct PagedAppendParams {
+  PagedCache c;
+  const void* k;      // new rows (batch, head, token strides)
+  const void* v;
+  const void* q;      // optional: rotated into q_out
+  void* q_out;
+  const float* cos;   // [capacity or more, rotary / 2], rows rot_ss apart
+  const float* sin;
+  int64_t k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, q_sb, q_sh, q_ss, qo_sb, qo_sh, qo_ss;
+  int64_t cos_ss, sin_ss;
+  int rotary, interleaved;
+  int pages_per_seq;  // store blocks per sequence (each walks the touched pages this far apart)
+};
+
+// Attention over the pages (fal_paged.hip).
+struct PagedAttnParams {
+  PagedCache c;
+  const void* q;
+  void* o;
+  float* lse;         // optional [total, Hq]
+  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
+  float scale_log2;   // |softmax_scale| * log2(e), at least 1e-30
+  int negate_q;
+  int causal;
+};
+
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);
 int fwd_block_m(int d);
 bool fwd_pipe_ok(int d);   // batched calls of this head dim run the pipelined tile loop
@@ -195,5 +246,8 @@ hipError_t launch_bwd_dq(const BwdParams& p, int d, int causal, dim3 grid, hipSt
 int decode_chunk(int d, int B, int Hkv, int max_seqlen);
 
 hipError_t launch_decode(const DecodeParams& p, int d, hipStream_t st);
+
+hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st);
+hipError_t launch_paged_attn(const PagedAttnParams& p, int d, hipStream_t st);
 
 }  // namespace fal

@@ -43,6 +43,9 @@ struct Api {
   decltype(&fal_bwd) bwd[2];
   decltype(&fal_bwd_varlen) bwd_varlen[2];
   decltype(&fal_decode) decode[2];
+  decltype(&fal_paged_append) paged_append[2];
+  decltype(&fal_paged_attn) paged_attn[2];
+  decltype(&fal_paged_attn_workspace_size) paged_attn_ws;
 } api;
 
 [[noreturn]] void fail(const std::string& msg) { throw std::runtime_error(msg); }
@@ -271,6 +274,154 @@ std::vector<Tensor> decode(Tensor q, Tensor k, Tensor v, Tensor lens, double sca
   return {o};
 }
 
+// ---- paged cache ---------------------------------------------------------------------------
+
+// Tensors whose addresses a fal_paged_cache holds (converted copies among them).
+struct Paged {
+  fal_paged_cache c{};
+  Tensor table, lens, cu;
+};
+
+void check_device(const char* name, const Tensor& t, const Tensor& like) {
+  if (t.device() != like.device())
+    fail(std::string(name) + " must be on " + like.device().str() + ", got " + t.device().str());
+}
+
+Tensor ints_on(const Tensor& t, const Tensor& like) {
+  return t.scalar_type() == at::kInt && t.device() == like.device() ? t : t.to(like.device(), at::kInt);
+}
+
+// x: the call's 16-bit tensor [B, n, H, d], or packed [total, H, d] with cu; hq and hkv its heads.
+// head_axis: 1 for caches [pages, Hkv, page_size, d], 2 for [pages, page_size, Hkv, d].
+Paged paged(const char* name, const Tensor& x, int64_t hq, const Tensor& kc, const Tensor& vc, const Tensor& ks,
+            const Tensor& vs, const Tensor& table, const Tensor& lens, const Tensor& cu, int64_t max_seqlen,
+            int64_t head_axis) {
+  Paged r;
+  fal_paged_cache& c = r.c;
+  if (cu.defined()) {
+    if (x.dim() != 3) fail(std::string(name) + " must be [total, heads, d] with cu_seqlens, got " + shape_str(x.sizes()));
+    require(cu.dim() == 1 && cu.size(0) >= 1, "cu_seqlens must be a 1-D tensor of batch + 1 offsets");
+    require(max_seqlen >= 0, "max_seqlen must not be negative");
+    c.batch = cu.size(0) - 1, c.seqlen = max_seqlen, c.total_tokens = x.size(0);
+  } else {
+    if (x.dim() != 4) fail(std::string(name) + " must be [B, n, heads, d] without cu_seqlens, got " + shape_str(x.sizes()));
+    c.batch = x.size(0), c.seqlen = x.size(1), c.total_tokens = c.batch * c.seqlen;
+  }
+  const int64_t d = x.size(-1);
+  check_device("k_cache", kc, x), check_device("v_cache", vc, x);
+  const at::ScalarType type = kc.scalar_type();
+  c.fp8 = type == at::kFloat8_e4m3fn;
+  if (vc.scalar_type() != type || (!c.fp8 && type != x.scalar_type()))
+    fail("k_cache and v_cache must both be float8_e4m3fn, or both of the type of " + std::string(name));
+  require(kc.dim() == 4 && vc.dim() == 4, "k_cache and v_cache must be 4-D");
+  require(kc.sizes() == vc.sizes() && kc.size(3) == d, "k_cache / v_cache shape mismatch");
+  require(kc.stride(3) == 1 && vc.stride(3) == 1, "k_cache and v_cache must be contiguous in the head dimension");
+  c.heads_q = hq, c.heads_kv = kc.size(head_axis), c.head_dim = d;
+  c.num_pages = kc.size(0), c.page_size = kc.size(3 - head_axis);
+  if (c.fp8) {
+    for (const Tensor* s : {&ks, &vs}) {
+      require(s->defined(), "a float8 cache needs k_scale and v_scale");
+      if (s->scalar_type() != at::kFloat || s->sizes() != at::IntArrayRef({c.num_pages, c.heads_kv}))
+        fail("k_scale and v_scale must be float32 " + shape_str({c.num_pages, c.heads_kv}) + ", got " +
+             std::string(c10::toString(s->scalar_type())) + " " + shape_str(s->sizes()));
+      check_device("k_scale and v_scale", *s, x);
+    }
+    c.k_scale = floats(ks), c.v_scale = floats(vs);
+    for (int i = 0; i < 2; ++i) c.k_scale_strides[i] = ks.stride(i), c.v_scale_strides[i] = vs.stride(i);
+  } else {
+    require(!ks.defined() && !vs.defined(), "k_scale and v_scale are for float8 caches");
+  }
+  if (table.dim() != 2 || table.size(0) != c.batch)
+    fail("page_table must be [" + std::to_string(c.batch) + ", max_pages], got " + shape_str(table.sizes()));
+  if (lens.numel() != c.batch)
+    fail("cache_seqlens must hold " + std::to_string(c.batch) + " lengths, got " + std::to_string(lens.numel()));
+  r.table = ints_on(table, x);
+  if (r.table.stride(1) != 1) r.table = r.table.contiguous();
+  r.lens = ints_on(lens, x);
+  if (r.lens.dim() != 1 || !r.lens.is_contiguous()) r.lens = r.lens.reshape({-1}).contiguous();
+  if (cu.defined()) r.cu = ints_on(cu, x).contiguous();
+  c.k = kc.data_ptr(), c.v = vc.data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    const int axis = i == 0 ? 0 : i == 1 ? (int)head_axis : 3 - (int)head_axis;
+    c.k_strides[i] = kc.stride(axis), c.v_strides[i] = vc.stride(axis);
+  }
+  c.page_table = ints(r.table), c.table_stride = r.table.stride(0), c.max_pages = r.table.size(1);
+  c.cache_seqlens = ints(r.lens), c.cu_seqlens = r.cu.defined() ? ints(r.cu) : nullptr;
+  return r;
+}
+
+// (batch, head, token) strides of [B, n, H, d]; (unused, head, token) of [total, H, d]
+Strides tokens(const Tensor& t) {
+  return t.dim() == 4 ? Strides{t.stride(0), t.stride(2), t.stride(1)} : Strides{0, t.stride(1), t.stride(0)};
+}
+
+// A table of fp32 rows that start on 16 bytes
+Tensor rotary_table(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) % 4 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.contiguous();
+}
+
+std::vector<Tensor> paged_append(Tensor k, Tensor v, Tensor kc, Tensor vc, Tensor table, Tensor lens, Tensor ks, Tensor vs,
+                                 Tensor q, Tensor cu, int64_t max_seqlen, Tensor cos, Tensor sin, bool interleaved,
+                                 int64_t head_axis) {
+  check_half_cuda("k", k);
+  if (v.scalar_type() != k.scalar_type() || v.device() != k.device() || v.sizes() != k.sizes())
+    fail("v must have the type, device and shape of k");
+  require(k.dim() >= 3, "k must be [B, n, H_kv, d], or [total, H_kv, d] with cu_seqlens");
+  const int64_t hkv = k.size(-2);
+  if (q.defined()) {
+    bool ok = q.scalar_type() == k.scalar_type() && q.device() == k.device() && q.dim() == k.dim() && q.size(-1) == k.size(-1);
+    for (int64_t i = 0; ok && i < k.dim() - 2; ++i) ok = q.size(i) == k.size(i);
+    require(ok, "q must have the type, device, tokens and head_dim of k");
+  }
+  const c10::DeviceGuard guard(k.device());
+  Paged p = paged("k", k, q.defined() ? q.size(-2) : hkv, kc, vc, ks, vs, table, lens, cu, max_seqlen, head_axis);
+  require(p.c.heads_kv == hkv, "k and k_cache have different numbers of heads");
+  int64_t rotary = 0;
+  require(cos.defined() == sin.defined(), "rotary_cos and rotary_sin go together");
+  if (cos.defined()) {
+    require(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, "rotary_cos and rotary_sin must be float32");
+    require(cos.dim() == 2 && cos.sizes() == sin.sizes(), "rotary_cos and rotary_sin must both be [positions, rotary_dim / 2]");
+    check_device("rotary_cos", cos, k), check_device("rotary_sin", sin, k);
+    cos = rotary_table(cos), sin = rotary_table(sin);
+    rotary = 2 * cos.size(1);
+  }
+  k = usable(k), v = usable(v);
+  Tensor out;
+  Strides qs{}, os{};
+  if (q.defined()) {
+    q = usable(q);
+    out = at::empty(q.sizes(), q.options());
+    qs = tokens(q), os = tokens(out);
+  }
+  const Strides kst = tokens(k), vst = tokens(v);
+  check_status(api.paged_append[bf16(k)](
+      &p.c, k.data_ptr(), v.data_ptr(), q.defined() ? q.data_ptr() : nullptr, q.defined() ? out.data_ptr() : nullptr,
+      kst.data(), vst.data(), qs.data(), os.data(), rotary ? floats(cos) : nullptr, rotary ? floats(sin) : nullptr,
+      rotary ? cos.size(0) : 0, rotary ? cos.stride(0) : 0, rotary ? sin.stride(0) : 0, rotary, interleaved, stream(k)));
+  if (q.defined()) return {out};
+  return {};
+}
+
+std::vector<Tensor> paged_attention(Tensor q, Tensor kc, Tensor vc, Tensor table, Tensor lens, Tensor ks, Tensor vs,
+                                    Tensor cu, int64_t max_seqlen, double scale, bool causal, int64_t head_axis,
+                                    bool want_lse) {
+  check_half_cuda("q", q);
+  require(q.dim() >= 3, "q must be [B, n, H_q, d], or [total, H_q, d] with cu_seqlens");
+  const c10::DeviceGuard guard(q.device());
+  const Paged p = paged("q", q, q.size(-2), kc, vc, ks, vs, table, lens, cu, max_seqlen, head_axis);
+  q = usable(q);
+  Tensor o = at::empty(q.sizes(), q.options()), l;
+  if (want_lse) l = at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat));
+  const size_t nws = api.paged_attn_ws(&p.c);
+  Tensor ws;
+  if (nws) ws = workspace(nws, q);
+  const Strides qs = tokens(q), os = tokens(o);
+  check_status(api.paged_attn[bf16(q)](&p.c, q.data_ptr(), o.data_ptr(), want_lse ? floats(l) : nullptr, qs.data(),
+                                       os.data(), (float)scale, causal, nws ? ws.data_ptr() : nullptr, nws, stream(q)));
+  if (want_lse) return {o, l};
+  return {o};
+}
+
 // ---------------------------------------------------------------------------
 // Python side: positional arguments only (hip_ext.py has the signatures).  The GIL is
 // released while the call runs, as ctypes does.
@@ -398,6 +549,50 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args x{a, n};
+  x.count(15);
+  Tensor k = x.tensor(0), v = x.tensor(1), kc = x.tensor(2), vc = x.tensor(3), table = x.tensor(4), lens = x.tensor(5),
+         ks = x.optional(6), vs = x.optional(7), q = x.optional(8), cu = x.optional(9);
+  const int64_t max_seqlen = x.integer(10);
+  Tensor cos = x.optional(11), sin = x.optional(12);
+  const bool interleaved = x.integer(13) != 0;
+  const int64_t head_axis = x.integer(14);
+  require(head_axis == 1 || head_axis == 2, "head axis must be 1 or 2");
+  std::vector<Tensor> r;
+  {
+    NoGil nogil;
+    r = paged_append(std::move(k), std::move(v), std::move(kc), std::move(vc), std::move(table), std::move(lens),
+                     std::move(ks), std::move(vs), std::move(q), std::move(cu), max_seqlen, std::move(cos),
+                     std::move(sin), interleaved, head_axis);
+  }
+  return to_list(r);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args x{a, n};
+  x.count(13);
+  Tensor q = x.tensor(0), kc = x.tensor(1), vc = x.tensor(2), table = x.tensor(3), lens = x.tensor(4), ks = x.optional(5),
+         vs = x.optional(6), cu = x.optional(7);
+  const int64_t max_seqlen = x.integer(8);
+  const double scale = x.number(9);
+  const bool causal = x.integer(10) != 0;
+  const int64_t head_axis = x.integer(11);
+  require(head_axis == 1 || head_axis == 2, "head axis must be 1 or 2");
+  const bool want_lse = x.integer(12) != 0;
+  std::vector<Tensor> r;
+  {
+    NoGil nogil;
+    r = paged_attention(std::move(q), std::move(kc), std::move(vc), std::move(table), std::move(lens), std::move(ks),
+                        std::move(vs), std::move(cu), max_seqlen, scale, causal, head_axis, want_lse);
+  }
+  return to_list(r);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}): the library's entry points
 PyObject* py_bind(PyObject*, PyObject* table) {
   HANDLE_TH_ERRORS
@@ -419,6 +614,9 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   set(api.bwd[0], "fal_bwd"), set(api.bwd[1], "fal_bwd_bf16");
   set(api.bwd_varlen[0], "fal_bwd_varlen"), set(api.bwd_varlen[1], "fal_bwd_varlen_bf16");
   set(api.decode[0], "fal_decode"), set(api.decode[1], "fal_decode_bf16");
+  set(api.paged_append[0], "fal_paged_append"), set(api.paged_append[1], "fal_paged_append_bf16");
+  set(api.paged_attn[0], "fal_paged_attn"), set(api.paged_attn[1], "fal_paged_attn_bf16");
+  set(api.paged_attn_ws, "fal_paged_attn_workspace_size");
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -430,6 +628,8 @@ PyMethodDef methods[] = {
     {"backward", (PyCFunction)(void*)py_backward, METH_FASTCALL, nullptr},
     {"backward_varlen", (PyCFunction)(void*)py_backward_varlen, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction)(void*)py_decode, METH_FASTCALL, nullptr},
+    {"paged_append", (PyCFunction)(void*)py_paged_append, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void*)py_paged_attention, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fal_torch", nullptr, -1, methods};

@@ -6,7 +6,7 @@ Drop-in for the ``flash_attn_legacy`` package: same functions, modules and
 HuggingFace registration, computed by hand-written HIP kernels for CDNA4.
 
 Supports MHA, GQA (grouped-query) and MQA (multi-query) attention; packed
-variable-length sequences; KV-cache decode.
+variable-length sequences; KV-cache decode; a paged KV cache in 16 or 8 bits.
 
 Head dimensions: 32, 64, 96, 128, 256
 
@@ -29,6 +29,12 @@ from .flash_attn import (
     FlashMultiHeadAttention,
 )
 
+from .paged import (
+    flash_attn_with_paged_kvcache,
+    paged_kvcache_append,
+    rotary_cos_sin,
+)
+
 from .utils import (
     check_gpu_compatibility,
     get_device_info,
@@ -40,6 +46,9 @@ __all__ = [
     "flash_attention",
     "flash_attn_varlen_func",
     "flash_attn_with_kvcache",
+    "flash_attn_with_paged_kvcache",
+    "paged_kvcache_append",
+    "rotary_cos_sin",
     "FlashAttention",
     "FlashMultiHeadAttention",
     "check_gpu_compatibility",

@@ -9,11 +9,13 @@ error behaviour (``RuntimeError`` with the library's message):
   softmax_scale, is_causal=False) -> [O, L]``
 * ``backward(dO, Q, K, V, O, L, softmax_scale, is_causal=False) -> [dQ, dK, dV]``
 
-plus two entry points the reference does not have:
+plus entry points the reference does not have:
 
 * ``backward_varlen(...)`` -- one launch for all packed sequences;
 * ``decode(q, k_cache, v_cache, cache_seqlens, softmax_scale, ...)`` -- split-K
-  KV-cache decode.
+  KV-cache decode;
+* ``paged_append(...)``, ``paged_attention(...)`` -- rotation and append to a paged cache in 16
+  or 8 bits, and attention to it.
 
 Outputs and workspaces are allocated with torch on the input's device; the library itself
 never allocates.  Work is enqueued on the current torch stream.  Both steps are native
@@ -49,6 +51,15 @@ _SZ = ctypes.c_size_t
 _STR = ctypes.c_void_p   # int64[3] stride triples
 
 
+class PagedCache(ctypes.Structure):
+    """``fal_paged_cache`` of fal_api.h."""
+    _fields_ = [(n, _VP) for n in ("k", "v", "k_scale", "v_scale", "page_table", "cache_seqlens", "cu_seqlens")] + [
+        ("k_strides", _I64 * 3), ("v_strides", _I64 * 3), ("k_scale_strides", _I64 * 2), ("v_scale_strides", _I64 * 2),
+        *[(n, _I64) for n in ("table_stride", "batch", "seqlen", "total_tokens", "heads_q", "heads_kv", "head_dim",
+                              "num_pages", "page_size", "max_pages")], ("fp8", ctypes.c_int32)]
+
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -73,7 +84,12 @@ def _load() -> ctypes.CDLL:
         "fal_decode": (_INT, [_VP] * 5 + [_I64, _VP, _VP] + [_I64] * 5 + [_STR] * 4 + [_F32, _VP, _SZ, _VP]),
         "fal_decode_noalloc": (_INT, [_VP] * 5 + [_I64, _VP, _VP] + [_I64] * 5 + [_STR] * 4 + [_F32, _VP]),
     }
-    for name in ("fal_fwd", "fal_fwd_varlen", "fal_bwd", "fal_bwd_varlen", "fal_decode"):
+    cache = ctypes.POINTER(PagedCache)
+    sig["fal_paged_append"] = (_INT, [cache] + [_VP] * 4 + [_STR] * 4 + [_VP] * 2 + [_I64] * 4 + [_INT, _VP])
+    sig["fal_paged_attn"] = (_INT, [cache] + [_VP] * 3 + [_STR] * 2 + [_F32, _INT, _VP, _SZ, _VP])
+    sig["fal_paged_attn_workspace_size"] = (_SZ, [cache])
+    for name in ("fal_fwd", "fal_fwd_varlen", "fal_bwd", "fal_bwd_varlen", "fal_decode", "fal_paged_append",
+                 "fal_paged_attn"):
         sig[name + "_bf16"] = sig[name]   # bf16 forms: same arguments
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -92,6 +108,8 @@ SYMBOLS = (
     "fal_decode_workspace_size", "fal_decode",
     "fal_fwd_bf16", "fal_fwd_varlen_bf16", "fal_bwd_bf16", "fal_bwd_varlen_bf16", "fal_decode_bf16",
     "fal_decode_noalloc",
+    "fal_paged_append", "fal_paged_append_bf16", "fal_paged_attn", "fal_paged_attn_bf16",
+    "fal_paged_attn_workspace_size",
 )
 
 
@@ -159,8 +177,36 @@ def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cache_
     """Split-K decode.  q [B,Hq,d] (one token per sequence); caches [B,S,Hkv,d]
     (``cache_layout="bshd"``) or [B,Hkv,S,d] (``"bhsd"``); cache_seqlens int32 [B];
     mask_bias optional fp32 [B,S] additive mask.  Returns O [B,Hq,d] (and L [B,Hq])."""
+    axis = _head_axis(cache_layout)
+    res = _native.decode(q, k_cache, v_cache, cache_seqlens, float(softmax_scale), mask_bias, axis, bool(return_lse))
+    return tuple(res) if return_lse else res[0]
+
+
+def _head_axis(cache_layout: str) -> int:
     axis = _HEAD_AXIS.get(cache_layout)
     if axis is None:
         raise RuntimeError(f"unknown cache_layout {cache_layout!r}")
-    res = _native.decode(q, k_cache, v_cache, cache_seqlens, float(softmax_scale), mask_bias, axis, bool(return_lse))
+    return axis
+
+
+def paged_append(k, v, k_cache, v_cache, page_table, cache_seqlens, k_scale=None, v_scale=None, q=None,
+                 cu_seqlens=None, max_seqlen: int = 0, rotary_cos=None, rotary_sin=None, interleaved: bool = False,
+                 cache_layout: str = "bshd") -> Optional[torch.Tensor]:
+    """Rotate and append k, v [B,n,Hkv,d] (or packed [total,Hkv,d] with cu_seqlens) to the caches
+    [pages,page_size,Hkv,d] (``"bshd"``) or [pages,Hkv,page_size,d] (``"bhsd"``), in place.
+    Returns the rotated q, if there is one.  Contract: fal_paged_append in fal_api.h."""
+    res = _native.paged_append(k, v, k_cache, v_cache, page_table, cache_seqlens, k_scale, v_scale, q, cu_seqlens,
+                               int(max_seqlen), rotary_cos, rotary_sin, bool(interleaved), _head_axis(cache_layout))
+    return res[0] if res else None
+
+
+def paged_attention(q, k_cache, v_cache, page_table, cache_seqlens, softmax_scale: float, k_scale=None, v_scale=None,
+                    cu_seqlens=None, max_seqlen: int = 0, is_causal: bool = True, cache_layout: str = "bshd",
+                    return_lse: bool = False):
+    """Attention of q [B,n,Hq,d] (or packed [total,Hq,d] with cu_seqlens), the last tokens of
+    each sequence, to its pages.  Returns O in q's shape (and L without the last axis).
+    Contract: fal_paged_attn in fal_api.h."""
+    res = _native.paged_attention(q, k_cache, v_cache, page_table, cache_seqlens, k_scale, v_scale, cu_seqlens,
+                                  int(max_seqlen), float(softmax_scale), bool(is_causal), _head_axis(cache_layout),
+                                  bool(return_lse))
     return tuple(res) if return_lse else res[0]

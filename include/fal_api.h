@@ -252,6 +252,83 @@ int fal_decode_noalloc(const void* q, const void* k_cache, const void* v_cache,
                        const int64_t* v_strides, const int64_t* o_strides,
                        float softmax_scale, void* stream);
 
+/*
+ * Paged KV cache.  No counterpart in the reference.
+ * A cache is a pool of num_pages pages of page_size rows (a multiple of 16); row i of sequence b
+ * is row i % page_size of page page_table[b][i / page_size].  Pages outside [0, num_pages) are
+ * never touched: an append drops their rows, attention skips them.
+ *   - fp8 0: elements of the call's 16-bit type, no scales (NULL).  fp8 1: e4m3 codes (OCP,
+ *     finite and NaN), and a row's value is code * scale of its page and KV head.
+ *   - tokens, the rows of k, v, q and o: with cu_seqlens, packed tensors of total_tokens rows, of
+ *     which sequence b owns cu_seqlens[b] .. cu_seqlens[b + 1]; their strides are (unused, head,
+ *     token), and seqlen, the longest sequence, only sizes the grid (a longer one is right, but
+ *     slower).  Without it, seqlen tokens in each sequence, total_tokens = batch * seqlen, strides
+ *     (batch, head, token).
+ */
+typedef struct fal_paged_cache {
+  void* k;                        /* 16-byte aligned */
+  void* v;
+  float* k_scale;                 /* fp32, entry (page, head) at page * strides[0] + head * strides[1] */
+  float* v_scale;
+  const int32_t* page_table;      /* device int32 [batch, max_pages], rows table_stride apart */
+  const int32_t* cache_seqlens;   /* device int32 [batch] */
+  const int32_t* cu_seqlens;      /* device int32 [batch + 1], or NULL */
+  int64_t k_strides[3];           /* elements: page, head, row; multiples of 16 bytes */
+  int64_t v_strides[3];
+  int64_t k_scale_strides[2];
+  int64_t v_scale_strides[2];
+  int64_t table_stride;
+  int64_t batch, seqlen, total_tokens;
+  int64_t heads_q, heads_kv, head_dim;
+  int64_t num_pages, page_size, max_pages;   /* max_pages * page_size < 2^31 */
+  int32_t fp8;
+} fal_paged_cache;
+
+/*
+ * Rotate and append.  Token i of sequence b becomes row cache_seqlens[b] + i of its cache
+ * (cache_seqlens: rows before the append); rows past max_pages * page_size are dropped.
+ *   k, v [tokens, Hkv, d]; q [tokens, Hq, d], optional (NULL), is rotated into q_out (rows
+ *   outside every sequence and dropped ones come back zero).
+ *   rotary_dim: the first rotary_dim elements (a multiple of 16; 0: no rotation, NULL tables) of
+ *   q and k are rotated by the angles of the row's position p, whose cosines and sines are rows p
+ *   of the fp32 tables [rotary_rows, rotary_dim / 2], rotary_rows >= max_pages * page_size, in
+ *   pairs (j, j + rotary_dim / 2) or, interleaved, (2j, 2j + 1).  Products and sums in fp32.
+ *   16-bit caches get the row rounded once.  8-bit caches: the scale of a touched (page, head)
+ *   becomes the smallest power of two s >= 2^-126 with 448 s >= every finite magnitude of the
+ *   rows that the call puts there, or stays, if it is larger and the page held rows of the
+ *   sequence before; where it grows, those rows' codes are rounded to the new scale.  Values
+ *   are rounded to e4m3 in units of the scale; infinities become the largest code, NaN stays.
+ * A page that is written must belong to one sequence.  No workspace.
+ */
+int fal_paged_append(const fal_paged_cache* cache, const void* k, const void* v, const void* q, void* q_out,
+                     const int64_t* k_strides, const int64_t* v_strides,
+                     const int64_t* q_strides, const int64_t* q_out_strides,
+                     const float* rotary_cos, const float* rotary_sin, int64_t rotary_rows,
+                     int64_t cos_stride, int64_t sin_stride, int64_t rotary_dim, int rotary_interleaved,
+                     void* stream);
+int fal_paged_append_bf16(const fal_paged_cache* cache, const void* k, const void* v, const void* q, void* q_out,
+                          const int64_t* k_strides, const int64_t* v_strides,
+                          const int64_t* q_strides, const int64_t* q_out_strides,
+                          const float* rotary_cos, const float* rotary_sin, int64_t rotary_rows,
+                          int64_t cos_stride, int64_t sin_stride, int64_t rotary_dim, int rotary_interleaved,
+                          void* stream);
+
+/*
+ * Attention of each sequence's last tokens to its cache, cache_seqlens[b] rows with those of the
+ * tokens themselves.  Causal: the last token sees every row and token i of n sees the rows
+ * j <= cache_seqlens[b] - n + i (bottom-right alignment); otherwise every token sees all rows.
+ *   q, o [tokens, Hq, d]; lse, optional, fp32 [tokens, Hq] contiguous, natural log.  A token that
+ *   sees no row, and a row outside every sequence, gets o = 0 and lse = -infinity.
+ * workspace: fal_paged_attn_workspace_size bytes (it reads the sizes and fp8 alone).
+ */
+size_t fal_paged_attn_workspace_size(const fal_paged_cache* cache);
+int fal_paged_attn(const fal_paged_cache* cache, const void* q, void* o, float* lse,
+                   const int64_t* q_strides, const int64_t* o_strides, float softmax_scale, int is_causal,
+                   void* workspace, size_t workspace_bytes, void* stream);
+int fal_paged_attn_bf16(const fal_paged_cache* cache, const void* q, void* o, float* lse,
+                        const int64_t* q_strides, const int64_t* o_strides, float softmax_scale, int is_causal,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
