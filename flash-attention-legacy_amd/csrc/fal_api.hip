@@ -874,8 +874,8 @@ int fill_paged(PagedCache& p, const fal_paged_cache* cache, int bf16, bool writt
                 (long long)c.heads_kv);
   if (c.page_size <= 0 || c.page_size % 16 != 0 || c.page_size > (1 << 16))
     return fail(FAL_ERR_UNSUPPORTED, "page_size must be a multiple of 16 up to 65536, got %lld", (long long)c.page_size);
-  if (c.max_pages < 0 || c.max_pages > 0x7fffffff / c.page_size)
-    return fail(FAL_ERR_INVALID, "page_table: max_pages * page_size must stay below 2^31");
+  if (c.max_pages < 0 || c.max_pages > (1 << 30) / c.page_size)
+    return fail(FAL_ERR_INVALID, "page_table: max_pages * page_size must not pass 2^30");
   if (!c.cu_seqlens && c.total_tokens != c.batch * c.seqlen)
     return fail(FAL_ERR_INVALID, "total_tokens must be batch * seqlen");
   if (c.batch == 0 && c.total_tokens > 0) return fail(FAL_ERR_INVALID, "tokens without a sequence");
@@ -957,6 +957,11 @@ int paged_append_impl(const fal_paged_cache* cache, const void* k, const void* v
   return launch_status(launch_paged_append(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_append");
 }
 
+PagedPlan plan_of(const fal_paged_cache& c) {
+  return paged_plan(c.batch, c.seqlen, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim,
+                    c.cu_seqlens != nullptr);
+}
+
 int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
                     const int64_t* o_strides, float softmax_scale, int is_causal, void* workspace,
                     size_t workspace_bytes, void* stream, int bf16) {
@@ -976,7 +981,15 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   p.scale_log2 = scale_log2(softmax_scale);
   p.negate_q = softmax_scale < 0.f;
   p.causal = is_causal != 0;
-  if (c.total_tokens * c.heads_q > 0x7fffffff) return fail(FAL_ERR_INVALID, "problem too large for one launch");
+  const PagedPlan plan = plan_of(c);
+  p.chunk = plan.chunk, p.max_splits = plan.max_splits, p.nc = plan.nc, p.col_tiles = plan.col_tiles;
+  p.direct = plan.direct;
+  const size_t parts = (size_t)c.total_tokens * c.heads_q * plan.max_splits;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(parts * c.head_dim * sizeof(float)));
+  if (c.total_tokens * c.heads_q > 0x7fffffff ||
+      c.batch * c.heads_kv > 0x7fffffff / ((int64_t)plan.max_splits * plan.col_tiles))
+    return fail(FAL_ERR_INVALID, "problem too large for one launch");
   return launch_status(launch_paged_attn(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_attn");
 }
 
@@ -1002,8 +1015,15 @@ int fal_paged_append_bf16(const fal_paged_cache* cache, const void* k, const voi
 }
 
 size_t fal_paged_attn_workspace_size(const fal_paged_cache* cache) {
-  (void)cache;
-  return 0;
+  if (!cache) return 0;
+  const fal_paged_cache& c = *cache;
+  if (c.heads_q <= 0 || c.heads_kv <= 0 || c.heads_q % c.heads_kv != 0 || !dims_ok(c.batch) || !dims_ok(c.seqlen) ||
+      !dims_ok(c.total_tokens) || c.page_size <= 0 || c.max_pages < 0 || c.max_pages > (1 << 30) / c.page_size)
+    return 0;
+  const PagedPlan plan = plan_of(c);
+  if (plan.direct) return 0;
+  const size_t parts = (size_t)c.total_tokens * c.heads_q * plan.max_splits;
+  return align256(parts * c.head_dim * sizeof(float)) + align256(parts * sizeof(float));
 }
 int fal_paged_attn(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
                    const int64_t* o_strides, float softmax_scale, int is_causal, void* workspace,

@@ -302,93 +302,479 @@ hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st
 }
 
 // ---------------------------------------------------------------------------
-// Attention: one workgroup per (token, query head), one wave per four rows
+// Attention, few columns: split over the rows
 // ---------------------------------------------------------------------------
-template <class T, bool FP8>
-__device__ __forceinline__ float cache_elem(const void* row, int e) {
-  if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[e], 0);
-  else return (float)((const T*)row)[e];
+// A column is one (token, query head) of a KV head: column c of a sequence is token c / G and
+// head c % G of the group of G heads.  One workgroup takes NC tiles of 16 columns and `chunk`
+// cache rows of one sequence and KV head; its four waves take 32-row steps in turn, each as two
+// slices of 16 rows (a slice lies in one page), with no barrier until the final merge.
+// * S^T = K Q^T on 16x16x32 MFMA, M = 16 rows, N = 16 columns: every K and V byte is read once
+//   for all columns of the tile.
+// * K rows go straight to registers in MFMA order, two steps ahead; e4m3 codes become 16-bit
+//   values there (exact in both types).  V rows go through a wave-private LDS ring by direct
+//   copies and come back transposed (ds_read_b64_tr_b16 / _tr_b8) as the operand of
+//   O^T = V^T P^T.
+// * A page's key scale multiplies its scores.  Its value scale multiplies P relative to the
+//   largest seen so far, which O is kept in units of, so P stays in [0, 1] and no 16-bit value
+//   leaves its type's range whatever the scales are.
+// Bound by reading the cache.
+constexpr int kPagedWaves = 4;
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt_n() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// Combine with the lanes 16 and 32 apart.
+__device__ __forceinline__ float quarters_max(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return pair_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return pair_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+}
+
+// Eight e4m3 codes as 16-bit values (exact)
+template <class T>
+__device__ __forceinline__ vec8<T> e4m3_to_16(uint32_t lo, uint32_t hi) {
+  u32x4 r;
+  if constexpr (std::is_same<T, half_t>::value) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true));
+  } else {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  }
+  return __builtin_bit_cast(vec8<T>, r);
+}
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+// Transposed LDS read of bytes: within 16 lanes, which read 8 rows x 16 columns (lane i row i / 2,
+// columns 8 (i % 2) .. + 8), lane r gets column r, row j in byte j.
+__device__ __forceinline__ u32x2 lds_tr8(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) i32x2 lds_i2;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(p)));
+}
+
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
+__device__ __forceinline__ float lane_of(float x, int lane) { return __uint_as_float(lane_of(__float_as_uint(x), lane)); }
+
+// Slice layout of V in LDS: 16 rows in 16-byte chunks, chunk index XOR-swizzled by the row so
+// that a transposed read, whose half wave takes 8 rows of both slices, spreads over all banks.
+template <bool FP8, int D>
+struct VSlice {
+  static constexpr int RB = FP8 ? D : 2 * D;                 // bytes of a row
+  static constexpr int CPR = RB / 16;
+  static constexpr int LOADS = (16 * CPR + 63) / 64;         // direct copies of 64 chunks
+  static constexpr int BYTES = LOADS * 1024;                 // (a last half-used copy pads)
+  __device__ static int swz(int row, int slice) {
+    if (D == 96) return FP8 ? 0 : row & 3;
+    if (!FP8) return row & (CPR < 16 ? CPR - 1 : 15);
+    constexpr int RPL = CPR < 16 ? 16 / CPR : 1;             // rows per 256 bytes
+    return (row / RPL + slice * (8 / RPL)) & (CPR - 1);
+  }
+};
+
+// A pair of K pieces loaded by lines -> MFMA order.  Loaded: a = (lane n < 8 of a row of 16
+// lanes: row n piece 0; n >= 8: row n - 8 piece 1), b = the same of rows 8 .. 15.  Wanted:
+// a = row n piece 0, b = row n piece 1.  Lanes 8-15 of a take b from 8 lanes below, lanes 0-7 of
+// b take a from 8 lanes above (row_ror:8).
+__device__ __forceinline__ void unswap_lines(u32x4& a, u32x4& b) {
+  u32x4 na, nb;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    na[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)a[i], (int)b[i], 0x128, 0xf, 0xc, false);
+    nb[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)b[i], (int)a[i], 0x128, 0xf, 0x3, false);
+  }
+  a = na, b = nb;
+}
+
+template <class T, bool FP8, int D, int NC>
+__global__ void __launch_bounds__(kPagedWaves * 64)
+paged_split_kernel(PagedAttnParams p) {
+  constexpr int NW = kPagedWaves;
+  constexpr int KS = D / 32;                     // 32-wide k-steps over the head dim
+  constexpr int DBN = D / 16;
+  using VS = VSlice<FP8, D>;
+  // K registers of a slice: 16-byte pieces that cover 64 bytes of each of its 16 rows
+  constexpr int KL = FP8 ? D / 64 : D / 32, KTAIL = FP8 ? (D % 64) / 32 : 0;   // (tail: 32 bytes of each row)
+  constexpr bool LINE = KL >= 2;                 // pairs of pieces loaded as whole 128-byte lines
+  constexpr int LPS = 2 * (KL + KTAIL + VS::LOADS);
+  using V8 = vec8<T>;
+  __shared__ __attribute__((aligned(1024))) uint8_t vsm[NW][4 * VS::BYTES];   // 2 steps x 2 slices
+  __shared__ float m_s[NW][16], l_s[NW][16], inv_s[16];
+  static_assert(sizeof(vsm[0]) >= 16 * D * sizeof(float), "a wave's ring holds its partial O");
+
+  const PagedCache& c = p.c;
+  const int G = c.Hq / c.Hkv;
+  int rest = blockIdx.x;
+  const int ct0 = rest % p.col_tiles;
+  rest /= p.col_tiles;
+  const int hkv = rest % c.Hkv;
+  rest /= c.Hkv;
+  const int b = rest % c.B, split = rest / c.B;
+  const int L = min(max(c.seqlens[b], 0), c.capacity);
+  const int k_begin = split * p.chunk;
+  if (k_begin >= L && split > 0) return;
+  int off, len;
+  token_range(c, b, off, len);
+  const int k_end = min(L, k_begin + p.chunk);
+  const int nsteps = cdiv(k_end - k_begin, 32);
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = tid >> 6;
+  const int ws = __builtin_amdgcn_readfirstlane(w);
+  const int l16 = lane & 15;
+  const int g4 = lane >> 4;
+
+  // This wave's slices, one per lane: slice i is half i % 2 of step ws + NW * (i / 2).  Byte
+  // offsets of its first rows, the rows it has (0: none, or a page outside the pool) and its scales.
+  constexpr int CB = FP8 ? 1 : 2;
+  int64_t koff = 0, voff = 0;
+  int nrow = 0;
+  float ksc = 1.f, vsc = 1.f;
+  {
+    const int r = k_begin + (ws + NW * (lane >> 1)) * 32 + (lane & 1) * 16;
+    if (r < k_end) {
+      const int page = r / c.page_size, slot = r - page * c.page_size;
+      const int pid = c.table[b * c.table_sb + page];
+      if (pid >= 0 && pid < c.num_pages) {
+        nrow = min(16, k_end - r);
+        koff = (pid * c.k_sp + hkv * c.k_sh + slot * c.k_ss) * CB;
+        voff = (pid * c.v_sp + hkv * c.v_sh + slot * c.v_ss) * CB;
+        if (FP8) {
+          ksc = c.k_scale[pid * c.ks_sp + hkv * c.ks_sh];
+          vsc = c.v_scale[pid * c.vs_sp + hkv * c.vs_sh];
+        }
+      }
+    }
+  }
+  const int k_ss = (int)c.k_ss * CB, v_ss = (int)c.v_ss * CB;   // row strides in bytes (below 2^23)
+  // K: 16 bytes g4 of row l16 in piece t, or, by lines, of row l16 % 8 (+ 8 in the second of a
+  // pair) and piece t + l16 / 8 (kline order; see unswap)
+  const int kv0 = l16 * k_ss + g4 * 16;
+  const int kvl = (l16 & 7) * k_ss + (g4 + 4 * (l16 >> 3)) * 16;
+  int vv[2][VS::LOADS];   // byte of the chunk that each copy brings to this lane's place in a slice
+#pragma unroll
+  for (int I = 0; I < VS::LOADS; ++I) {
+    const int q = I * 64 + lane, r = q / VS::CPR;
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl)   // (past the slice's 16 rows: outside the resource, nothing is read)
+      vv[sl][I] = r < 16 ? r * v_ss + ((q % VS::CPR) ^ VS::swz(r, sl)) * 16 : 0x7ffffff0;
+  }
+  uint8_t* const ring = &vsm[ws][0];
+
+  u32x4 kreg[2][2][KL > 0 ? KL : 1];
+  u32x2 ktail[2][2];
+  auto issue = [&](int jj, int buf) {   // the wave's step jj
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl) {
+      const int i = 2 * jj + sl;
+      const int n = (int)lane_of((uint32_t)nrow, i);
+      const int64_t ko = (int64_t)(((uint64_t)lane_of((uint32_t)(koff >> 32), i) << 32) | lane_of((uint32_t)koff, i));
+      const int64_t vo = (int64_t)(((uint64_t)lane_of((uint32_t)(voff >> 32), i) << 32) | lane_of((uint32_t)voff, i));
+      const auto krs = make_rsrc((const char*)c.k + ko, n > 0 ? (uint32_t)((n - 1) * k_ss + D * CB) : 0);
+      const auto vrs = make_rsrc((const char*)c.v + vo, n > 0 ? (uint32_t)((n - 1) * v_ss + D * CB) : 0);
+#pragma unroll
+      for (int t = 0; t < KL; ++t) {
+        const bool pair = LINE && (t | 1) < KL;
+        // whole lines are read once and evicted first; halves stay until the other half is read
+        kreg[buf][sl][t] = pair ? __builtin_amdgcn_raw_buffer_load_b128(krs, kvl + (t & 1) * 8 * k_ss + (t & ~1) * 64, 0, 2)
+                                : __builtin_amdgcn_raw_buffer_load_b128(krs, kv0 + t * 64, 0, 0);
+      }
+      if constexpr (KTAIL)
+        ktail[buf][sl] = __builtin_amdgcn_raw_buffer_load_b64(krs, l16 * k_ss + KL * 64 + g4 * 8, 0, 0);
+#pragma unroll
+      for (int I = 0; I < VS::LOADS; ++I)
+        buffer_to_lds16<2>(vrs, vv[sl][I], ring + (buf * 2 + sl) * VS::BYTES + I * 1024);
+    }
+  };
+
+  // transposed V reads
+  constexpr int VROW = VS::RB;
+  const int kk = l16 >> 1;                                   // e4m3: row kk of the 8, slice kk / 4
+  const int vr = FP8 ? 4 * g4 + (kk & 3) : 4 * g4 + (l16 >> 2);
+  const uint8_t* vbase = FP8 ? ring + (kk >> 2) * VS::BYTES + vr * VROW + 8 * (l16 & 1) : ring + vr * VROW + 8 * (l16 & 1);
+  const int vc0 = FP8 ? VS::swz(vr, kk >> 2) : ((l16 >> 1) & 1) ^ VS::swz(vr, 0);
+
+  const int ncols = len * G;
+  for (int ct = ct0; ct * NC * 16 < ncols; ct += p.col_tiles) {
+    int j = ws;          // this wave's steps: ws, ws + NW, ...
+    if (j < nsteps) issue(0, 0);
+    if (j + NW < nsteps) issue(1, 1);
+
+    // queries of the columns as the B operand (n = column, k = head dim in K's order)
+    V8 qreg[NC][KS];
+    int lim[NC];         // rows below this one are seen by the column
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      const int col = (ct * NC + nc) * 16 + l16;
+      const int i = col / G, h = hkv * G + col % G;
+      const T* qrow = (const T*)p.q + (c.cu ? (int64_t)(off + i) * p.q_ss : b * p.q_sb + i * p.q_ss) + h * p.q_sh;
+      lim[nc] = p.causal ? L - len + i + 1 : L;
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        const int e = FP8 && t < 2 * KL ? (t >> 1) * 64 + g4 * 16 + (t & 1) * 8 : t * 32 + g4 * 8;
+        qreg[nc][t] = col < ncols ? ld8(qrow + e) : zero8<T>();
+        if (p.negate_q) qreg[nc][t] = -qreg[nc][t];
+      }
+    }
+    f32x4 oacc[NC][DBN];
+    float m_run[NC], l_run[NC];
+    float ref = 0.f;     // value scale that O is in units of
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      m_run[nc] = -INFINITY, l_run[nc] = 0.f;
+#pragma unroll
+      for (int i = 0; i < DBN; ++i) oacc[nc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto step = [&](auto bufc, int jj) {
+      constexpr int buf = decltype(bufc)::value;
+      if (j + NW < nsteps) wait_vmcnt_n<LPS>();
+      else wait_vmcnt_n<0>();
+      f32x4 s[NC][2];
+      float vfac[2], back = 1.f;
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {
+        V8 kop[KS];
+        if constexpr (LINE) {
+#pragma unroll
+          for (int t = 0; t + 1 < KL; t += 2) unswap_lines(kreg[buf][sl][t], kreg[buf][sl][t + 1]);
+        }
+        if constexpr (FP8) {
+#pragma unroll
+          for (int t = 0; t < KL; ++t) {
+            kop[2 * t] = e4m3_to_16<T>(kreg[buf][sl][t][0], kreg[buf][sl][t][1]);
+            kop[2 * t + 1] = e4m3_to_16<T>(kreg[buf][sl][t][2], kreg[buf][sl][t][3]);
+          }
+          if constexpr (KTAIL) kop[KS - 1] = e4m3_to_16<T>(ktail[buf][sl][0], ktail[buf][sl][1]);
+        } else {
+#pragma unroll
+          for (int t = 0; t < KS; ++t) kop[t] = __builtin_bit_cast(V8, kreg[buf][sl][t]);
+        }
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+          s[nc][sl] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < KS; ++t) s[nc][sl] = mfma16(kop[t], qreg[nc][t], s[nc][sl]);
+        }
+      }
+      const int n0 = (int)lane_of((uint32_t)nrow, 2 * jj), n1 = (int)lane_of((uint32_t)nrow, 2 * jj + 1);
+      float kfac[2] = {p.scale_log2, p.scale_log2};
+      if constexpr (FP8) {
+        kfac[0] *= lane_of(ksc, 2 * jj), kfac[1] *= lane_of(ksc, 2 * jj + 1);
+        const float v0 = n0 > 0 ? lane_of(vsc, 2 * jj) : 0.f, v1 = n1 > 0 ? lane_of(vsc, 2 * jj + 1) : 0.f;
+        const float now = fmaxf(ref, fmaxf(v0, v1));
+        const float inv = now >= 0x1p-126f ? __builtin_amdgcn_rcpf(now) : 0.f;
+        vfac[0] = v0 * inv, vfac[1] = v1 * inv, back = ref * inv;
+        ref = now;
+      }
+      V8 pb[NC];
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        const int r0 = k_begin + j * 32 + 4 * g4;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool seen = 4 * g4 + i < (sl ? n1 : n0) && r0 + sl * 16 + i < lim[nc];
+            const float x = seen ? s[nc][sl][i] * kfac[sl] : -INFINITY;
+            s[nc][sl][i] = x;
+            mx = fmaxf(mx, x);
+          }
+        mx = quarters_max(mx);
+        const float m_new = fmaxf(m_run[nc], mx);
+        const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
+        const float alpha = fast_exp2(m_run[nc] - m_use);
+        m_run[nc] = m_new;
+        float l = l_run[nc] * alpha;
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = fast_exp2(s[nc][sl][i] - m_use);
+            l += e;
+            pb[nc][sl * 4 + i] = (T)(FP8 ? e * vfac[sl] : e);
+          }
+        l_run[nc] = l;
+        const float f = FP8 ? alpha * back : alpha;
+#pragma unroll
+        for (int db = 0; db < DBN; ++db) oacc[nc][db] *= f;
+      }
+      // O^T += V^T P^T over the 32 rows
+#pragma unroll
+      for (int db = 0; db < DBN; ++db) {
+        V8 vop;
+        if constexpr (FP8) {
+          const u32x2 x = lds_tr8(vbase + buf * 2 * VS::BYTES + ((db ^ vc0) << 4));
+          vop = e4m3_to_16<T>(x[0], x[1]);
+        } else {
+          const T* v0 = (const T*)(vbase + buf * 2 * VS::BYTES + ((vc0 ^ (2 * db)) << 4));
+          vop = join8(lds_tr(v0), lds_tr((const T*)((const uint8_t*)v0 + VS::BYTES)));
+        }
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) oacc[nc][db] = mfma16(vop, pb[nc], oacc[nc][db]);
+      }
+      // LDS reads of this buffer must finish before the next copies overwrite it
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (j + 2 * NW < nsteps) issue(jj + 2, buf);
+      j += NW;
+    };
+    // two steps per trip so that the ring index is a compile-time constant
+    for (int jj = 0; j < nsteps; jj += 2) {
+      step(std::integral_constant<int, 0>{}, jj);
+      if (j >= nsteps) break;
+      step(std::integral_constant<int, 1>{}, jj + 1);
+    }
+
+    // ---- merge the waves in a fixed order; each tile of columns in turn ----
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      const float l_tot = quarters_sum(l_run[nc]);
+      if (lane < 16) {
+        m_s[w][l16] = m_run[nc];
+        l_s[w][l16] = l_tot;
+      }
+      __syncthreads();
+      float M = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) M = fmaxf(M, m_s[i][l16]);
+      const float M_use = (M == -INFINITY) ? 0.f : M;
+      const float wscale = fast_exp2(m_run[nc] - M_use) * (FP8 ? ref : 1.f);
+      float* part = reinterpret_cast<float*>(ring);   // (the wave's ring is idle)
+#pragma unroll
+      for (int db = 0; db < DBN; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[l16 * D + db * 16 + 4 * g4 + i] = oacc[nc][db][i] * wscale;
+      const int col0 = (ct * NC + nc) * 16;
+      const int nh = min(16, ncols - col0);
+      // partial (token, head, split); token row t of head h is t * Hq + h
+      auto row_of = [&](int n) {
+        const int col = col0 + n;
+        return (int64_t)((c.cu ? off : b * c.n) + col / G) * c.Hq + hkv * G + col % G;
+      };
+      if (w == 0 && lane < nh) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) sum += l_s[i][l16] * fast_exp2(m_s[i][l16] - M_use);
+        inv_s[l16] = sum > 0.f ? 1.f / sum : 0.f;
+        const float lse2 = sum > 0.f ? M_use + fast_log2(sum) : -INFINITY;
+        if (!p.direct) p.part_m[row_of(l16) * p.max_splits + split] = lse2;
+        else if (p.lse) p.lse[row_of(l16)] = lse2 * kLn2;
+      }
+      __syncthreads();
+      for (int i = tid; i < nh * D; i += NW * 64) {
+        const int n = i / D, d = i % D;
+        float o = 0.f;
+#pragma unroll
+        for (int ww = 0; ww < NW; ++ww) o += reinterpret_cast<const float*>(&vsm[ww][0])[n * D + d];
+        o *= inv_s[n];
+        if (!p.direct) {
+          p.part_o[(row_of(n) * p.max_splits + split) * D + d] = o;
+        } else {
+          const int col = col0 + n, t = col / G;
+          T* orow = (T*)p.o + (c.cu ? (int64_t)(off + t) * p.o_ss : b * p.o_sb + t * p.o_ss) + (hkv * G + col % G) * p.o_sh;
+          orow[d] = (T)o;
+        }
+      }
+      __syncthreads();   // before the ring and the statistics are written again
+    }
+  }
+}
+
+// One wave per (token, query head): merge the splits' partial outputs, sixteen per round trip.
+template <class T, int D>
+__global__ void __launch_bounds__(64)
+paged_combine_kernel(PagedAttnParams p) {
+  const PagedCache& c = p.c;
+  const int h = blockIdx.x % c.Hq, t = blockIdx.x / c.Hq;
+  const int lane = threadIdx.x;
+  int b = 0, i = 0, ns = 0;
+  if (token_place(c, t, b, i)) ns = cdiv(min(max(c.seqlens[b], 0), c.capacity), p.chunk);
+  const int64_t row = (int64_t)t * c.Hq + h, base = row * p.max_splits;
+  constexpr int DJ = (D + 63) / 64;
+  constexpr int CH = 16;
+  float acc[DJ];
+#pragma unroll
+  for (int j = 0; j < DJ; ++j) acc[j] = 0.f;
+  float M = -INFINITY, wsum = 0.f;
+  for (int s0 = 0; s0 < ns; s0 += CH) {
+    float pm[CH], x[CH][DJ];
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const bool ok = s0 + u < ns;
+      pm[u] = ok ? p.part_m[base + s0 + u] : -INFINITY;
+      const float* po = p.part_o + (base + s0 + u) * D;
+#pragma unroll
+      for (int j = 0; j < DJ; ++j) x[u][j] = (ok && lane + 64 * j < D) ? po[lane + 64 * j] : 0.f;
+    }
+    float cm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) cm = fmaxf(cm, pm[u]);
+    const float Mn = fmaxf(M, cm);
+    if (Mn == -INFINITY) continue;
+    const float r = fast_exp2(M - Mn);
+    wsum *= r;
+#pragma unroll
+    for (int j = 0; j < DJ; ++j) acc[j] *= r;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const float wgt = fast_exp2(pm[u] - Mn);
+      wsum += wgt;
+#pragma unroll
+      for (int j = 0; j < DJ; ++j) acc[j] = fmaf(wgt, x[u][j], acc[j]);
+    }
+    M = Mn;
+  }
+  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
+#pragma unroll
+  for (int j = 0; j < DJ; ++j) {
+    const int d = lane + 64 * j;
+    if (d < D) orow[d] = (T)(acc[j] * inv);
+  }
+  if (p.lse && lane == 0) p.lse[row] = wsum > 0.f ? (M + fast_log2(wsum)) * kLn2 : -INFINITY;
+}
+
+// Rows per split: halve from 2048 until the longest sequences' splits are four workgroups per
+// compute unit.
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool packed) {
+  PagedPlan r{};
+  const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
+  r.nc = cols <= 16 || d > 128 ? 1 : 2;   // (head dim 256: two tiles would not fit the registers)
+  const int64_t tiles = (cols + 16 * r.nc - 1) / (16 * r.nc);
+  r.col_tiles = (int)(tiles < 4096 ? tiles : 4096);
+  const int64_t rows = capacity > 0 ? capacity : 1;
+  int chunk = 2048;
+  while (chunk > kPagedWaves * 32 && B * Hkv * r.col_tiles * ((rows + chunk - 1) / chunk) < 1024) chunk >>= 1;
+  r.chunk = chunk;
+  r.max_splits = (int)((rows + chunk - 1) / chunk);
+  r.direct = r.max_splits == 1 && !packed;
+  return r;
 }
 
 template <class T, bool FP8, int D>
-__global__ void __launch_bounds__(256)
-paged_attn_simple_kernel(PagedAttnParams p) {
-  const PagedCache& c = p.c;
-  constexpr int CB = FP8 ? 1 : 2, DJ = (D + 63) / 64;
-  __shared__ float m_s[4], l_s[4], o_s[4][D];
-  const int t = blockIdx.x / c.Hq, h = blockIdx.x % c.Hq, hk = h / (c.Hq / c.Hkv);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int b = 0, i = 0, off = 0, len = 0, end = 0;
-  if (token_place(c, t, b, i)) {
-    token_range(c, b, off, len);
-    const int L = min(max(c.seqlens[b], 0), c.capacity);
-    end = p.causal ? max(L - len + i + 1, 0) : L;
-  }
-  const T* qrow = (const T*)p.q + (c.cu ? t * p.q_ss : b * p.q_sb + i * p.q_ss) + h * p.q_sh;
-  T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
-  float q[DJ], o[DJ];
-#pragma unroll
-  for (int j = 0; j < DJ; ++j) {
-    const int e = lane + 64 * j;
-    q[j] = e < D ? (float)qrow[e] * (p.negate_q ? -p.scale_log2 : p.scale_log2) : 0.f;
-    o[j] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int r = w; r < end; r += 4) {
-    const int pid = c.table[b * c.table_sb + r / c.page_size];
-    if (pid < 0 || pid >= c.num_pages) continue;
-    const char* k = (const char*)c.k + (pid * c.k_sp + hk * c.k_sh + (r % c.page_size) * c.k_ss) * CB;
-    const char* v = (const char*)c.v + (pid * c.v_sp + hk * c.v_sh + (r % c.page_size) * c.v_ss) * CB;
-    float x = 0.f;
-#pragma unroll
-    for (int j = 0; j < DJ; ++j)
-      if (lane + 64 * j < D) x = fmaf(q[j], cache_elem<T, FP8>(k, lane + 64 * j), x);
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
-    if (FP8) x *= c.k_scale[pid * c.ks_sp + hk * c.ks_sh];
-    const float mn = fmaxf(m, x), use = mn == -INFINITY ? 0.f : mn;
-    const float a = fast_exp2(m - use), e = fast_exp2(x - use);
-    m = mn;
-    l = l * a + e;
-    const float ev = FP8 ? e * c.v_scale[pid * c.vs_sp + hk * c.vs_sh] : e;
-#pragma unroll
-    for (int j = 0; j < DJ; ++j)
-      if (lane + 64 * j < D) o[j] = fmaf(ev, cache_elem<T, FP8>(v, lane + 64 * j), o[j] * a);
-  }
-  if (lane == 0) m_s[w] = m, l_s[w] = l;
-#pragma unroll
-  for (int j = 0; j < DJ; ++j)
-    if (lane + 64 * j < D) o_s[w][lane + 64 * j] = o[j];
-  __syncthreads();
-  if (w) return;
-  const float M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-  const float use = M == -INFINITY ? 0.f : M;
-  float total = 0.f;
-  for (int x = 0; x < 4; ++x) total += l_s[x] * fast_exp2(m_s[x] - use);
-  const float inv = total > 0.f ? 1.f / total : 0.f;
-#pragma unroll
-  for (int j = 0; j < DJ; ++j) {
-    const int e = lane + 64 * j;
-    float acc = 0.f;
-    if (e < D) {
-      for (int x = 0; x < 4; ++x) acc += o_s[x][e] * fast_exp2(m_s[x] - use);
-      orow[e] = (T)(acc * inv);
-    }
-  }
-  if (p.lse && lane == 0) p.lse[(int64_t)t * c.Hq + h] = total > 0.f ? (use + fast_log2(total)) * kLn2 : -INFINITY;
+static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)p.max_splits * p.c.B * p.c.Hkv * p.col_tiles)), block(kPagedWaves * 64);
+  if (D > 128 || p.nc == 1) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((paged_split_kernel<T, FP8, (D > 128 ? 128 : D), 2>), grid, block, 0, st, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.direct) return e;
+  hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(64), 0, st, p);
+  return hipGetLastError();
 }
 
 template <int D>
 static hipError_t launch_attn_d(const PagedAttnParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)p.c.total * p.c.Hq));
-  if (p.c.fp8) {
-    if (p.c.bf16) hipLaunchKernelGGL((paged_attn_simple_kernel<bf16_t, true, D>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((paged_attn_simple_kernel<half_t, true, D>), grid, dim3(256), 0, st, p);
-  } else {
-    if (p.c.bf16) hipLaunchKernelGGL((paged_attn_simple_kernel<bf16_t, false, D>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((paged_attn_simple_kernel<half_t, false, D>), grid, dim3(256), 0, st, p);
-  }
-  return hipGetLastError();
+  if (p.c.fp8) return p.c.bf16 ? launch_attn_t<bf16_t, true, D>(p, st) : launch_attn_t<half_t, true, D>(p, st);
+  return p.c.bf16 ? launch_attn_t<bf16_t, false, D>(p, st) : launch_attn_t<half_t, false, D>(p, st);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& p, int d, hipStream_t st) {

@@ -280,7 +280,7 @@ typedef struct fal_paged_cache {
   int64_t table_stride;
   int64_t batch, seqlen, total_tokens;
   int64_t heads_q, heads_kv, head_dim;
-  int64_t num_pages, page_size, max_pages;   /* max_pages * page_size < 2^31 */
+  int64_t num_pages, page_size, max_pages;   /* max_pages * page_size <= 2^30 */
   int32_t fp8;
 } fal_paged_cache;
 

@@ -60,7 +60,7 @@ BAD_CACHES = [
     (dict(batch=0, seqlen=1, total_tokens=2, cu_seqlens=P), FAL_ERR_INVALID, "tokens without a sequence"),
     (dict(page_size=40), FAL_ERR_UNSUPPORTED, "page_size must be a multiple of 16"),
     (dict(page_size=0), FAL_ERR_UNSUPPORTED, "page_size must be a multiple of 16"),
-    (dict(max_pages=2 ** 25), FAL_ERR_INVALID, "must stay below 2^31"),
+    (dict(max_pages=2 ** 25), FAL_ERR_INVALID, "must not pass 2^30"),
     (dict(cache_seqlens=None), FAL_ERR_INVALID, "cache_seqlens: null pointer"),
     (dict(page_table=None), FAL_ERR_INVALID, "page_table: null pointer"),
     (dict(table_stride=-1), FAL_ERR_INVALID, "page_table: negative stride"),
