@@ -958,8 +958,11 @@ int paged_append_impl(const fal_paged_cache* cache, const void* k, const void* v
 }
 
 PagedPlan plan_of(const fal_paged_cache& c) {
+  // bytes that a head's row has for itself: a whole page where heads lie one after the other
+  const bool by_row = c.heads_kv > 1 && c.k_strides[1] < c.k_strides[2];
+  const int64_t row_bytes = (c.fp8 ? 1 : 2) * c.head_dim * (by_row ? 1 : c.page_size);
   return paged_plan(c.batch, c.seqlen, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim,
-                    c.cu_seqlens != nullptr);
+                    (int)std::min<int64_t>(row_bytes, 1 << 20), std::max(device_cu_count(), 1));
 }
 
 int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
@@ -982,13 +985,14 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   p.negate_q = softmax_scale < 0.f;
   p.causal = is_causal != 0;
   const PagedPlan plan = plan_of(c);
-  p.chunk = plan.chunk, p.max_splits = plan.max_splits, p.nc = plan.nc, p.col_tiles = plan.col_tiles;
-  p.direct = plan.direct;
-  const size_t parts = (size_t)c.total_tokens * c.heads_q * plan.max_splits;
+  p.parts = plan.parts, p.unit_rows = plan.unit_rows, p.wave_heads = plan.wave_heads;
+  p.nc = plan.nc, p.col_tiles = plan.col_tiles, p.cols = plan.cols;
+  const size_t rows = (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
   p.part_o = static_cast<float*>(workspace);
-  p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(parts * c.head_dim * sizeof(float)));
-  if (c.total_tokens * c.heads_q > 0x7fffffff ||
-      c.batch * c.heads_kv > 0x7fffffff / ((int64_t)plan.max_splits * plan.col_tiles))
+  p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(rows * c.head_dim * sizeof(float)));
+  if (c.total_tokens * c.heads_q > 0x7fffffff || c.seqlen * c.heads_q > 0x7fffffff ||
+      (int64_t)plan.parts * c.heads_kv * plan.col_tiles > 0x7fffffff ||
+      c.batch * ((c.max_pages * c.page_size + plan.unit_rows - 1) / plan.unit_rows) / plan.parts >= 0x7fffffff)
     return fail(FAL_ERR_INVALID, "problem too large for one launch");
   return launch_status(launch_paged_attn(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_attn");
 }
@@ -1021,9 +1025,8 @@ size_t fal_paged_attn_workspace_size(const fal_paged_cache* cache) {
       !dims_ok(c.total_tokens) || c.page_size <= 0 || c.max_pages < 0 || c.max_pages > (1 << 30) / c.page_size)
     return 0;
   const PagedPlan plan = plan_of(c);
-  if (plan.direct) return 0;
-  const size_t parts = (size_t)c.total_tokens * c.heads_q * plan.max_splits;
-  return align256(parts * c.head_dim * sizeof(float)) + align256(parts * sizeof(float));
+  const size_t rows = (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
+  return align256(rows * c.head_dim * sizeof(float)) + align256(rows * sizeof(float));
 }
 int fal_paged_attn(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
                    const int64_t* o_strides, float softmax_scale, int is_causal, void* workspace,

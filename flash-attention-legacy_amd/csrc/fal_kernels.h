@@ -184,14 +184,14 @@ struct PagedAttnParams {
   float scale_log2;   // |softmax_scale| * log2(e), at least 1e-30
   int negate_q;
   int causal;
-  // split kernel: each sequence's rows in chunks, one workgroup per (chunk, sequence, KV head,
-  // nc tiles of 16 columns); the partial outputs are merged unless `direct`
-  int chunk, max_splits, nc, col_tiles, direct;
-  float* part_o;      // [total, Hq, max_splits, d]
-  float* part_m;      // [total, Hq, max_splits] log2-domain LSE
+  // split kernel: the sequences' rows, in units of unit_rows, in `parts` equal runs; one workgroup
+  // per (run, wave_heads KV heads, nc tiles of 16 columns)
+  int parts, unit_rows, wave_heads, nc, col_tiles, cols;
+  float* part_o;      // [parts + B, Hkv, cols, d]
+  float* part_m;      // [parts + B, Hkv, cols] log2-domain LSE
 };
 struct PagedPlan {
-  int chunk, max_splits, nc, col_tiles, direct;
+  int parts, unit_rows, wave_heads, nc, col_tiles, cols;
 };
 
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);
@@ -257,6 +257,7 @@ hipError_t launch_decode(const DecodeParams& p, int d, hipStream_t st);
 
 hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st);
 hipError_t launch_paged_attn(const PagedAttnParams& p, int d, hipStream_t st);
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool packed);
+// row_bytes: bytes next to each other that belong to one KV head
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, int row_bytes, int ncu);
 
 }  // namespace fal

@@ -305,9 +305,15 @@ hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st
 // Attention, few columns: split over the rows
 // ---------------------------------------------------------------------------
 // A column is one (token, query head) of a KV head: column c of a sequence is token c / G and
-// head c % G of the group of G heads.  One workgroup takes NC tiles of 16 columns and `chunk`
-// cache rows of one sequence and KV head; its four waves take 32-row steps in turn, each as two
-// slices of 16 rows (a slice lies in one page), with no barrier until the final merge.
+// head c % G of the group of G heads.  The rows of all sequences, in units, are cut into `parts`
+// equal runs (see Runs); one workgroup takes one run for NC tiles of 16 columns and one, two or
+// four KV heads, and its four waves share the heads and then the rows: each takes 32-row steps
+// in turn, as two slices of 16 rows (a slice lies in one page), with no barrier until the merge
+// at the end of a sequence or of the run.
+// Equal runs: with fixed chunks of each sequence, 32 sequences of 1k to 32k rows left a tail of
+// half-empty rounds, and grids sized for the page table's capacity were mostly empty.
+// Several heads: rows of 128 bytes, one head's of many, reach 5.0 TB/s, four heads' side by side
+// RATE4 (32 sequences of 16k rows, 8 KV heads).
 // * S^T = K Q^T on 16x16x32 MFMA, M = 16 rows, N = 16 columns: every K and V byte is read once
 //   for all columns of the tile.
 // * K rows go straight to registers in MFMA order, two steps ahead; e4m3 codes become 16-bit
@@ -393,8 +399,40 @@ __device__ __forceinline__ void unswap_lines(u32x4& a, u32x4& b) {
   a = na, b = nb;
 }
 
+// The units of all sequences, in order, cut into `parts` runs whose lengths differ by one at
+// most: the first `extra` have `each` + 1.  Sequence b's units that lie in run g make up piece
+// g + b: along the order either g or b grows by one, so pieces are numbered without gaps.
+struct Runs {
+  int64_t each, extra;
+  __device__ Runs(int64_t units, int parts) {
+    if (units >> 31) each = units / parts;
+    else each = (uint32_t)units / (uint32_t)parts;
+    extra = units - each * parts;
+  }
+  __device__ int64_t begin(int g) const { return g * each + (g < extra ? g : extra); }
+  __device__ int of(int64_t unit) const {   // the run that a unit lies in
+    const int64_t head = extra * (each + 1);
+    if (unit < head) return (int)((unit >> 31) ? unit / (each + 1) : (uint32_t)unit / (uint32_t)(each + 1));
+    return (int)(extra + ((unit - head) >> 31 ? (unit - head) / each : (uint32_t)(unit - head) / (uint32_t)each));
+  }
+};
+
+__device__ __forceinline__ int cache_rows(const PagedCache& c, int b) { return min(max(c.seqlens[b], 0), c.capacity); }
+
+// Units of 64 sequences, one per lane, and their inclusive sums.
+__device__ __forceinline__ int lane_units(const PagedCache& c, int base, int unit_rows, int lane, int& sum) {
+  const int u = base + lane < c.B ? cdiv(cache_rows(c, base + lane), unit_rows) : 0;
+  sum = u;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(sum, o);
+    if (lane >= o) sum += t;
+  }
+  return u;
+}
+
 template <class T, bool FP8, int D, int NC>
-__global__ void __launch_bounds__(kPagedWaves * 64)
+__global__ void __launch_bounds__(kPagedWaves * 64, D > 128 ? 1 : 2)
 paged_split_kernel(PagedAttnParams p) {
   constexpr int NW = kPagedWaves;
   constexpr int KS = D / 32;                     // 32-wide k-steps over the head dim
@@ -406,54 +444,56 @@ paged_split_kernel(PagedAttnParams p) {
   constexpr int LPS = 2 * (KL + KTAIL + VS::LOADS);
   using V8 = vec8<T>;
   __shared__ __attribute__((aligned(1024))) uint8_t vsm[NW][4 * VS::BYTES];   // 2 steps x 2 slices
-  __shared__ float m_s[NW][16], l_s[NW][16], inv_s[16];
+  __shared__ float m_s[NW][16], l_s[NW][16], inv_s[NW][16];
   static_assert(sizeof(vsm[0]) >= 16 * D * sizeof(float), "a wave's ring holds its partial O");
 
   const PagedCache& c = p.c;
   const int G = c.Hq / c.Hkv;
-  int rest = blockIdx.x;
-  const int ct0 = rest % p.col_tiles;
-  rest /= p.col_tiles;
-  const int hkv = rest % c.Hkv;
-  rest /= c.Hkv;
-  const int b = rest % c.B, split = rest / c.B;
-  const int L = min(max(c.seqlens[b], 0), c.capacity);
-  const int k_begin = split * p.chunk;
-  if (k_begin >= L && split > 0) return;
-  int off, len;
-  token_range(c, b, off, len);
-  const int k_end = min(L, k_begin + p.chunk);
-  const int nsteps = cdiv(k_end - k_begin, 32);
-
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = tid >> 6;
   const int ws = __builtin_amdgcn_readfirstlane(w);
   const int l16 = lane & 15;
   const int g4 = lane >> 4;
+  int rest = blockIdx.x;
+  const int ct = rest % p.col_tiles;
+  rest /= p.col_tiles;
+  const int WH = p.wave_heads, NR = NW / WH;     // KV heads of the workgroup, waves on each
+  const int hgroup = rest % (c.Hkv / WH);
+  const int run = rest / (c.Hkv / WH);
+  const int hkv = hgroup * WH + ws % WH;
+  const int wr = ws / WH;
 
-  // This wave's slices, one per lane: slice i is half i % 2 of step ws + NW * (i / 2).  Byte
-  // offsets of its first rows, the rows it has (0: none, or a page outside the pool) and its scales.
-  constexpr int CB = FP8 ? 1 : 2;
-  int64_t koff = 0, voff = 0;
-  int nrow = 0;
-  float ksc = 1.f, vsc = 1.f;
+  // this run's first sequence and unit
+  int b = 0, local = 0, left;
   {
-    const int r = k_begin + (ws + NW * (lane >> 1)) * 32 + (lane & 1) * 16;
-    if (r < k_end) {
-      const int page = r / c.page_size, slot = r - page * c.page_size;
-      const int pid = c.table[b * c.table_sb + page];
-      if (pid >= 0 && pid < c.num_pages) {
-        nrow = min(16, k_end - r);
-        koff = (pid * c.k_sp + hkv * c.k_sh + slot * c.k_ss) * CB;
-        voff = (pid * c.v_sp + hkv * c.v_sh + slot * c.v_ss) * CB;
-        if (FP8) {
-          ksc = c.k_scale[pid * c.ks_sp + hkv * c.ks_sh];
-          vsc = c.v_scale[pid * c.vs_sp + hkv * c.vs_sh];
-        }
-      }
+    int sum, u = 0;
+    int64_t units = 0;
+    for (int base = 0; base < c.B; base += 64) {
+      u = lane_units(c, base, p.unit_rows, lane, sum);
+      units += __shfl(sum, 63);
     }
+    const Runs runs(units, p.parts);
+    const int64_t u0 = runs.begin(run);
+    left = __builtin_amdgcn_readfirstlane((int)(runs.begin(run + 1) - u0));
+    if (left <= 0) return;
+    int64_t before = 0;
+    for (int base = 0; base < c.B; base += 64) {
+      if (c.B > 64) u = lane_units(c, base, p.unit_rows, lane, sum);
+      const auto past = __ballot(before + sum > u0);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        b = base + at;
+        local = (int)(u0 - before) - (__shfl(sum, at) - __shfl(u, at));
+        break;
+      }
+      before += __shfl(sum, 63);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    local = __builtin_amdgcn_readfirstlane(local);
   }
+
+  constexpr int CB = FP8 ? 1 : 2;
   const int k_ss = (int)c.k_ss * CB, v_ss = (int)c.v_ss * CB;   // row strides in bytes (below 2^23)
   // K: 16 bytes g4 of row l16 in piece t, or, by lines, of row l16 % 8 (+ 8 in the second of a
   // pair) and piece t + l16 / 8 (kline order; see unswap)
@@ -471,30 +511,6 @@ paged_split_kernel(PagedAttnParams p) {
 
   u32x4 kreg[2][2][KL > 0 ? KL : 1];
   u32x2 ktail[2][2];
-  auto issue = [&](int jj, int buf) {   // the wave's step jj
-#pragma unroll
-    for (int sl = 0; sl < 2; ++sl) {
-      const int i = 2 * jj + sl;
-      const int n = (int)lane_of((uint32_t)nrow, i);
-      const int64_t ko = (int64_t)(((uint64_t)lane_of((uint32_t)(koff >> 32), i) << 32) | lane_of((uint32_t)koff, i));
-      const int64_t vo = (int64_t)(((uint64_t)lane_of((uint32_t)(voff >> 32), i) << 32) | lane_of((uint32_t)voff, i));
-      const auto krs = make_rsrc((const char*)c.k + ko, n > 0 ? (uint32_t)((n - 1) * k_ss + D * CB) : 0);
-      const auto vrs = make_rsrc((const char*)c.v + vo, n > 0 ? (uint32_t)((n - 1) * v_ss + D * CB) : 0);
-#pragma unroll
-      for (int t = 0; t < KL; ++t) {
-        const bool pair = LINE && (t | 1) < KL;
-        // whole lines are read once and evicted first; halves stay until the other half is read
-        kreg[buf][sl][t] = pair ? __builtin_amdgcn_raw_buffer_load_b128(krs, kvl + (t & 1) * 8 * k_ss + (t & ~1) * 64, 0, 2)
-                                : __builtin_amdgcn_raw_buffer_load_b128(krs, kv0 + t * 64, 0, 0);
-      }
-      if constexpr (KTAIL)
-        ktail[buf][sl] = __builtin_amdgcn_raw_buffer_load_b64(krs, l16 * k_ss + KL * 64 + g4 * 8, 0, 0);
-#pragma unroll
-      for (int I = 0; I < VS::LOADS; ++I)
-        buffer_to_lds16<2>(vrs, vv[sl][I], ring + (buf * 2 + sl) * VS::BYTES + I * 1024);
-    }
-  };
-
   // transposed V reads
   constexpr int VROW = VS::RB;
   const int kk = l16 >> 1;                                   // e4m3: row kk of the 8, slice kk / 4
@@ -502,11 +518,15 @@ paged_split_kernel(PagedAttnParams p) {
   const uint8_t* vbase = FP8 ? ring + (kk >> 2) * VS::BYTES + vr * VROW + 8 * (l16 & 1) : ring + vr * VROW + 8 * (l16 & 1);
   const int vc0 = FP8 ? VS::swz(vr, kk >> 2) : ((l16 >> 1) & 1) ^ VS::swz(vr, 0);
 
-  const int ncols = len * G;
-  for (int ct = ct0; ct * NC * 16 < ncols; ct += p.col_tiles) {
-    int j = ws;          // this wave's steps: ws, ws + NW, ...
-    if (j < nsteps) issue(0, 0);
-    if (j + NW < nsteps) issue(1, 1);
+  for (; left > 0; ++b, local = 0) {
+    const int L = cache_rows(c, b);
+    const int take = min(left, cdiv(L, p.unit_rows) - local);
+    left -= take;
+    const int row0 = local * p.unit_rows, row1 = min(L, (local + take) * p.unit_rows);
+    int off, len;
+    token_range(c, b, off, len);
+    const int ncols = min(len, c.n) * G;
+    if (row0 >= row1 || ct * NC * 16 >= ncols) continue;
 
     // queries of the columns as the B operand (n = column, k = head dim in K's order)
     V8 qreg[NC][KS];
@@ -534,9 +554,60 @@ paged_split_kernel(PagedAttnParams p) {
       for (int i = 0; i < DBN; ++i) oacc[nc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    // Blocks of rows whose slices fit a wave's lanes, one per lane: slice i is half i % 2 of step
+    // wr + NR * (i / 2).  Byte offsets of its first rows, the rows it has (0: none, or a page
+    // outside the pool) and its scales.
+    for (int k_begin = row0; k_begin < row1; k_begin += 1024 * NR) {
+    const int k_end = min(row1, k_begin + 1024 * NR);
+    const int nsteps = cdiv(k_end - k_begin, 32);
+    int64_t koff = 0, voff = 0;
+    int nrow = 0;
+    float ksc = 1.f, vsc = 1.f;
+    {
+      const int r = k_begin + (wr + NR * (lane >> 1)) * 32 + (lane & 1) * 16;
+      if (r < k_end) {
+        const int page = r / c.page_size, slot = r - page * c.page_size;
+        const int pid = c.table[b * c.table_sb + page];
+        if (pid >= 0 && pid < c.num_pages) {
+          nrow = min(16, k_end - r);
+          koff = (pid * c.k_sp + hkv * c.k_sh + slot * c.k_ss) * CB;
+          voff = (pid * c.v_sp + hkv * c.v_sh + slot * c.v_ss) * CB;
+          if (FP8) {
+            ksc = c.k_scale[pid * c.ks_sp + hkv * c.ks_sh];
+            vsc = c.v_scale[pid * c.vs_sp + hkv * c.vs_sh];
+          }
+        }
+      }
+    }
+    auto issue = [&](int jj, int buf) {   // the wave's step jj
+  #pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {
+        const int i = 2 * jj + sl;
+        const int n = (int)lane_of((uint32_t)nrow, i);
+        const int64_t ko = (int64_t)(((uint64_t)lane_of((uint32_t)(koff >> 32), i) << 32) | lane_of((uint32_t)koff, i));
+        const int64_t vo = (int64_t)(((uint64_t)lane_of((uint32_t)(voff >> 32), i) << 32) | lane_of((uint32_t)voff, i));
+        const auto krs = make_rsrc((const char*)c.k + ko, n > 0 ? (uint32_t)((n - 1) * k_ss + D * CB) : 0);
+        const auto vrs = make_rsrc((const char*)c.v + vo, n > 0 ? (uint32_t)((n - 1) * v_ss + D * CB) : 0);
+  #pragma unroll
+        for (int t = 0; t < KL; ++t) {
+          const bool pair = LINE && (t | 1) < KL;
+          // whole lines are read once and evicted first; halves stay until the other half is read
+          kreg[buf][sl][t] = pair ? __builtin_amdgcn_raw_buffer_load_b128(krs, kvl + (t & 1) * 8 * k_ss + (t & ~1) * 64, 0, 2)
+                                  : __builtin_amdgcn_raw_buffer_load_b128(krs, kv0 + t * 64, 0, 0);
+        }
+        if constexpr (KTAIL)
+          ktail[buf][sl] = __builtin_amdgcn_raw_buffer_load_b64(krs, l16 * k_ss + KL * 64 + g4 * 8, 0, 0);
+  #pragma unroll
+        for (int I = 0; I < VS::LOADS; ++I)
+          buffer_to_lds16<2>(vrs, vv[sl][I], ring + (buf * 2 + sl) * VS::BYTES + I * 1024);
+      }
+    };
+    int j = wr;          // this wave's steps: wr, wr + NR, ...
+    if (j < nsteps) issue(0, 0);
+    if (j + NR < nsteps) issue(1, 1);
     auto step = [&](auto bufc, int jj) {
       constexpr int buf = decltype(bufc)::value;
-      if (j + NW < nsteps) wait_vmcnt_n<LPS>();
+      if (j + NR < nsteps) wait_vmcnt_n<LPS>();
       else wait_vmcnt_n<0>();
       f32x4 s[NC][2];
       float vfac[2], back = 1.f;
@@ -624,8 +695,8 @@ paged_split_kernel(PagedAttnParams p) {
       }
       // LDS reads of this buffer must finish before the next copies overwrite it
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (j + 2 * NW < nsteps) issue(jj + 2, buf);
-      j += NW;
+      if (j + 2 * NR < nsteps) issue(jj + 2, buf);
+      j += NR;
     };
     // two steps per trip so that the ring index is a compile-time constant
     for (int jj = 0; j < nsteps; jj += 2) {
@@ -633,8 +704,9 @@ paged_split_kernel(PagedAttnParams p) {
       if (j >= nsteps) break;
       step(std::integral_constant<int, 1>{}, jj + 1);
     }
+    }
 
-    // ---- merge the waves in a fixed order; each tile of columns in turn ----
+    // ---- merge the waves of each head in a fixed order; each tile of columns in turn ----
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       const float l_tot = quarters_sum(l_run[nc]);
@@ -644,8 +716,7 @@ paged_split_kernel(PagedAttnParams p) {
       }
       __syncthreads();
       float M = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) M = fmaxf(M, m_s[i][l16]);
+      for (int r = 0; r < NR; ++r) M = fmaxf(M, m_s[ws % WH + r * WH][l16]);
       const float M_use = (M == -INFINITY) ? 0.f : M;
       const float wscale = fast_exp2(m_run[nc] - M_use) * (FP8 ? ref : 1.f);
       float* part = reinterpret_cast<float*>(ring);   // (the wave's ring is idle)
@@ -655,50 +726,104 @@ paged_split_kernel(PagedAttnParams p) {
         for (int i = 0; i < 4; ++i) part[l16 * D + db * 16 + 4 * g4 + i] = oacc[nc][db][i] * wscale;
       const int col0 = (ct * NC + nc) * 16;
       const int nh = min(16, ncols - col0);
-      // partial (token, head, split); token row t of head h is t * Hq + h
-      auto row_of = [&](int n) {
-        const int col = col0 + n;
-        return (int64_t)((c.cu ? off : b * c.n) + col / G) * c.Hq + hkv * G + col % G;
-      };
-      if (w == 0 && lane < nh) {
+      // partial of (piece, KV head, column)
+      auto part_row = [&](int n, int kv) { return ((int64_t)(run + b) * c.Hkv + kv) * p.cols + col0 + n; };
+      if (wr == 0 && lane < nh) {
         float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) sum += l_s[i][l16] * fast_exp2(m_s[i][l16] - M_use);
-        inv_s[l16] = sum > 0.f ? 1.f / sum : 0.f;
-        const float lse2 = sum > 0.f ? M_use + fast_log2(sum) : -INFINITY;
-        if (!p.direct) p.part_m[row_of(l16) * p.max_splits + split] = lse2;
-        else if (p.lse) p.lse[row_of(l16)] = lse2 * kLn2;
+        for (int r = 0; r < NR; ++r) sum += l_s[w + r * WH][l16] * fast_exp2(m_s[w + r * WH][l16] - M_use);
+        inv_s[w][l16] = sum > 0.f ? 1.f / sum : 0.f;
+        p.part_m[part_row(l16, hkv)] = sum > 0.f ? M_use + fast_log2(sum) : -INFINITY;
       }
       __syncthreads();
-      for (int i = tid; i < nh * D; i += NW * 64) {
-        const int n = i / D, d = i % D;
+      for (int i = tid; i < WH * nh * D; i += NW * 64) {
+        const int d = i % D, n = i / D % nh, k = i / D / nh;
         float o = 0.f;
-#pragma unroll
-        for (int ww = 0; ww < NW; ++ww) o += reinterpret_cast<const float*>(&vsm[ww][0])[n * D + d];
-        o *= inv_s[n];
-        if (!p.direct) {
-          p.part_o[(row_of(n) * p.max_splits + split) * D + d] = o;
-        } else {
-          const int col = col0 + n, t = col / G;
-          T* orow = (T*)p.o + (c.cu ? (int64_t)(off + t) * p.o_ss : b * p.o_sb + t * p.o_ss) + (hkv * G + col % G) * p.o_sh;
-          orow[d] = (T)o;
-        }
+        for (int r = 0; r < NR; ++r) o += reinterpret_cast<const float*>(&vsm[k + r * WH][0])[n * D + d];
+        p.part_o[part_row(n, hgroup * WH + k) * D + d] = o * inv_s[k][n];
       }
       __syncthreads();   // before the ring and the statistics are written again
     }
   }
 }
 
-// One wave per (token, query head): merge the splits' partial outputs, sixteen per round trip.
-template <class T, int D>
+// Attention of one token i and query head h of sequence b by one wave, row after row: for tokens
+// past the stated longest sequence, which the grid of the split kernel has no columns for.
+template <class T, bool FP8, int D>
+__device__ void attend_alone(const PagedAttnParams& p, int b, int i, int h, const T* qrow, float (&o)[(D + 63) / 64],
+                             float& m, float& l) {
+  const PagedCache& c = p.c;
+  constexpr int DJ = (D + 63) / 64, CB = FP8 ? 1 : 2;
+  const int lane = threadIdx.x & 63, hk = h / (c.Hq / c.Hkv);
+  auto elem = [&](const char* row, int e) {
+    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[e], 0);
+    else return (float)((const T*)row)[e];
+  };
+  float q[DJ];
+#pragma unroll
+  for (int j = 0; j < DJ; ++j) {
+    const int e = lane + 64 * j;
+    q[j] = e < D ? (float)qrow[e] * (p.negate_q ? -p.scale_log2 : p.scale_log2) : 0.f;
+    o[j] = 0.f;
+  }
+  int off, len;
+  token_range(c, b, off, len);
+  const int L = cache_rows(c, b), end = p.causal ? L - len + i + 1 : L;
+  m = -INFINITY, l = 0.f;
+  for (int r = 0; r < end; ++r) {
+    const int pid = c.table[b * c.table_sb + r / c.page_size], slot = r % c.page_size;
+    if (pid < 0 || pid >= c.num_pages) continue;
+    const char* k = (const char*)c.k + (pid * c.k_sp + hk * c.k_sh + slot * c.k_ss) * CB;
+    const char* v = (const char*)c.v + (pid * c.v_sp + hk * c.v_sh + slot * c.v_ss) * CB;
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < DJ; ++j)
+      if (lane + 64 * j < D) x = fmaf(q[j], elem(k, lane + 64 * j), x);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+    if (FP8) x *= c.k_scale[pid * c.ks_sp + hk * c.ks_sh];
+    const float mn = fmaxf(m, x), use = mn == -INFINITY ? 0.f : mn;
+    const float a = fast_exp2(m - use), e = fast_exp2(x - use);
+    m = mn;
+    l = l * a + e;
+    const float ev = FP8 ? e * c.v_scale[pid * c.vs_sp + hk * c.vs_sh] : e;
+#pragma unroll
+    for (int j = 0; j < DJ; ++j)
+      if (lane + 64 * j < D) o[j] = fmaf(ev, elem(v, lane + 64 * j), o[j] * a);
+  }
+}
+
+// One wave per (token, query head): merge the pieces' partial outputs, sixteen per round trip.
+template <class T, bool FP8, int D>
 __global__ void __launch_bounds__(64)
 paged_combine_kernel(PagedAttnParams p) {
   const PagedCache& c = p.c;
   const int h = blockIdx.x % c.Hq, t = blockIdx.x / c.Hq;
   const int lane = threadIdx.x;
   int b = 0, i = 0, ns = 0;
-  if (token_place(c, t, b, i)) ns = cdiv(min(max(c.seqlens[b], 0), c.capacity), p.chunk);
-  const int64_t row = (int64_t)t * c.Hq + h, base = row * p.max_splits;
+  const bool in = token_place(c, t, b, i);
+  const bool alone = in && i >= c.n;   // past the stated longest sequence
+  const int G = c.Hq / c.Hkv;
+  int64_t base = 0;
+  if (in && !alone) {   // this sequence's pieces
+    int64_t units = 0, first = 0;
+    int mine = 0;
+    for (int at = 0; at < c.B; at += 64) {
+      int sum;
+      const int u = lane_units(c, at, p.unit_rows, lane, sum);
+      if (b >= at && b < at + 64) {
+        mine = __shfl(u, b - at);
+        first = units + __shfl(sum, b - at) - mine;
+      }
+      units += __shfl(sum, 63);
+    }
+    if (mine > 0) {
+      const Runs runs(units, p.parts);
+      const int g0 = runs.of(first);
+      ns = runs.of(first + mine - 1) - g0 + 1;
+      base = ((int64_t)(g0 + b) * c.Hkv + h / G) * p.cols + i * G + h % G;
+    }
+  }
+  const int64_t row = (int64_t)t * c.Hq + h, step = (int64_t)c.Hkv * p.cols;
   constexpr int DJ = (D + 63) / 64;
   constexpr int CH = 16;
   float acc[DJ];
@@ -710,8 +835,8 @@ paged_combine_kernel(PagedAttnParams p) {
 #pragma unroll
     for (int u = 0; u < CH; ++u) {
       const bool ok = s0 + u < ns;
-      pm[u] = ok ? p.part_m[base + s0 + u] : -INFINITY;
-      const float* po = p.part_o + (base + s0 + u) * D;
+      pm[u] = ok ? p.part_m[base + (s0 + u) * step] : -INFINITY;
+      const float* po = p.part_o + (base + (s0 + u) * step) * D;
 #pragma unroll
       for (int j = 0; j < DJ; ++j) x[u][j] = (ok && lane + 64 * j < D) ? po[lane + 64 * j] : 0.f;
     }
@@ -733,6 +858,8 @@ paged_combine_kernel(PagedAttnParams p) {
     }
     M = Mn;
   }
+  if (alone)
+    attend_alone<T, FP8, D>(p, b, i, h, (const T*)p.q + t * p.q_ss + h * p.q_sh, acc, M, wsum);
   const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
   T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
 #pragma unroll
@@ -743,31 +870,40 @@ paged_combine_kernel(PagedAttnParams p) {
   if (p.lse && lane == 0) p.lse[row] = wsum > 0.f ? (M + fast_log2(wsum)) * kLn2 : -INFINITY;
 }
 
-// Rows per split: halve from 2048 until the longest sequences' splits are four workgroups per
-// compute unit.
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool packed) {
+#ifndef FAL_PAGED_PIECE
+#define FAL_PAGED_PIECE 512
+#endif
+#ifndef FAL_PAGED_WPC
+#define FAL_PAGED_WPC 3
+#endif
+#ifndef FAL_PAGED_UNIT
+#define FAL_PAGED_UNIT 64
+#endif
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, int row_bytes, int ncu) {
   PagedPlan r{};
   const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
   r.nc = cols <= 16 || d > 128 ? 1 : 2;   // (head dim 256: two tiles would not fit the registers)
-  const int64_t tiles = (cols + 16 * r.nc - 1) / (16 * r.nc);
-  r.col_tiles = (int)(tiles < 4096 ? tiles : 4096);
-  const int64_t rows = capacity > 0 ? capacity : 1;
-  int chunk = 2048;
-  while (chunk > kPagedWaves * 32 && B * Hkv * r.col_tiles * ((rows + chunk - 1) / chunk) < 1024) chunk >>= 1;
-  r.chunk = chunk;
-  r.max_splits = (int)((rows + chunk - 1) / chunk);
-  r.direct = r.max_splits == 1 && !packed;
+  r.col_tiles = (int)((cols + 16 * r.nc - 1) / (16 * r.nc));
+  r.cols = r.col_tiles * 16 * r.nc;
+  r.wave_heads = 1;
+  while (r.wave_heads < 4 && Hkv % (2 * r.wave_heads) == 0 && row_bytes * r.wave_heads < FAL_PAGED_PIECE) r.wave_heads *= 2;
+  // a unit: two steps, which are in flight together, for each wave
+  r.unit_rows = FAL_PAGED_UNIT * kPagedWaves / r.wave_heads;
+  const int64_t most = B * ((capacity + r.unit_rows - 1) / r.unit_rows);
+  int64_t parts = (int64_t)ncu * FAL_PAGED_WPC / (Hkv / r.wave_heads * r.col_tiles);
+  parts = parts < 1 ? 1 : parts > most ? most : parts;
+  r.parts = (int)(parts < 1 ? 1 : parts);
   return r;
 }
 
 template <class T, bool FP8, int D>
 static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)p.max_splits * p.c.B * p.c.Hkv * p.col_tiles)), block(kPagedWaves * 64);
+  const dim3 grid((unsigned)(p.parts * (p.c.Hkv / p.wave_heads) * p.col_tiles)), block(kPagedWaves * 64);
   if (D > 128 || p.nc == 1) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((paged_split_kernel<T, FP8, (D > 128 ? 128 : D), 2>), grid, block, 0, st, p);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.direct) return e;
-  hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(64), 0, st, p);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(64), 0, st, p);
   return hipGetLastError();
 }
 
