@@ -324,7 +324,8 @@ hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st
 //   largest seen so far, which O is kept in units of, so P stays in [0, 1] and no 16-bit value
 //   leaves its type's range whatever the scales are.
 // Bound by reading the cache.
-constexpr int kPagedWaves = 4;
+// Waves of a workgroup of the split kernel: eight where their rings fit the LDS.
+__host__ __device__ constexpr int paged_waves(int d, bool fp8) { return d <= 128 || fp8 ? 8 : 4; }
 
 template <int N>
 __device__ __forceinline__ void wait_vmcnt_n() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -419,22 +420,28 @@ struct Runs {
 
 __device__ __forceinline__ int cache_rows(const PagedCache& c, int b) { return min(max(c.seqlens[b], 0), c.capacity); }
 
+// Inclusive sum over the wave's lanes (row shifts, then the rows' last lanes broadcast)
+__device__ __forceinline__ int lanes_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31
+  return x;
+}
+
 // Units of 64 sequences, one per lane, and their inclusive sums.
 __device__ __forceinline__ int lane_units(const PagedCache& c, int base, int unit_rows, int lane, int& sum) {
   const int u = base + lane < c.B ? cdiv(cache_rows(c, base + lane), unit_rows) : 0;
-  sum = u;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(sum, o);
-    if (lane >= o) sum += t;
-  }
+  sum = lanes_scan(u);
   return u;
 }
 
 template <class T, bool FP8, int D, int NC>
-__global__ void __launch_bounds__(kPagedWaves * 64, D > 128 ? 1 : 2)
+__global__ void __launch_bounds__(paged_waves(D, FP8) * 64, paged_waves(D, FP8) / 4)
 paged_split_kernel(PagedAttnParams p) {
-  constexpr int NW = kPagedWaves;
+  constexpr int NW = paged_waves(D, FP8);
   constexpr int KS = D / 32;                     // 32-wide k-steps over the head dim
   constexpr int DBN = D / 16;
   using VS = VSlice<FP8, D>;
@@ -471,7 +478,7 @@ paged_split_kernel(PagedAttnParams p) {
     int64_t units = 0;
     for (int base = 0; base < c.B; base += 64) {
       u = lane_units(c, base, p.unit_rows, lane, sum);
-      units += __shfl(sum, 63);
+      units += (int)lane_of((uint32_t)sum, 63);
     }
     const Runs runs(units, p.parts);
     const int64_t u0 = runs.begin(run);
@@ -484,10 +491,10 @@ paged_split_kernel(PagedAttnParams p) {
       if (past) {
         const int at = __builtin_ctzll(past);
         b = base + at;
-        local = (int)(u0 - before) - (__shfl(sum, at) - __shfl(u, at));
+        local = (int)(u0 - before) - (int)(lane_of((uint32_t)sum, at) - lane_of((uint32_t)u, at));
         break;
       }
-      before += __shfl(sum, 63);
+      before += (int)lane_of((uint32_t)sum, 63);
     }
     b = __builtin_amdgcn_readfirstlane(b);
     local = __builtin_amdgcn_readfirstlane(local);
@@ -706,10 +713,25 @@ paged_split_kernel(PagedAttnParams p) {
     }
     }
 
-    // ---- merge the waves of each head in a fixed order; each tile of columns in turn ----
+    // ---- the piece's partial output, normalised, and its log2-domain LSE ----
+    const int64_t piece = (int64_t)(run + b) * c.Hkv;
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
+      const int col0 = (ct * NC + nc) * 16;
+      const int nh = min(16, ncols - col0);
       const float l_tot = quarters_sum(l_run[nc]);
+      if (NR == 1) {   // a wave has all of its head's rows
+        const float f = l_tot > 0.f ? (FP8 ? ref : 1.f) / l_tot : 0.f;
+        const int64_t row = (piece + hkv) * p.cols + col0 + l16;
+        if (l16 < nh) {
+#pragma unroll
+          for (int db = 0; db < DBN; ++db)
+            *reinterpret_cast<f32x4*>(p.part_o + row * D + db * 16 + 4 * g4) = oacc[nc][db] * f;
+          if (g4 == 0) p.part_m[row] = l_tot > 0.f ? m_run[nc] + fast_log2(l_tot) : -INFINITY;
+        }
+        continue;
+      }
+      // the waves of each head, added in their order; 16-byte chunks XOR-swizzled by the column
       if (lane < 16) {
         m_s[w][l16] = m_run[nc];
         l_s[w][l16] = l_tot;
@@ -719,27 +741,25 @@ paged_split_kernel(PagedAttnParams p) {
       for (int r = 0; r < NR; ++r) M = fmaxf(M, m_s[ws % WH + r * WH][l16]);
       const float M_use = (M == -INFINITY) ? 0.f : M;
       const float wscale = fast_exp2(m_run[nc] - M_use) * (FP8 ? ref : 1.f);
-      float* part = reinterpret_cast<float*>(ring);   // (the wave's ring is idle)
+      constexpr int SW = D / 4 >= 16 && D != 96 ? 15 : 7;
+      f32x4* part = reinterpret_cast<f32x4*>(ring);   // (the wave's ring is idle)
 #pragma unroll
-      for (int db = 0; db < DBN; ++db)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[l16 * D + db * 16 + 4 * g4 + i] = oacc[nc][db][i] * wscale;
-      const int col0 = (ct * NC + nc) * 16;
-      const int nh = min(16, ncols - col0);
-      // partial of (piece, KV head, column)
-      auto part_row = [&](int n, int kv) { return ((int64_t)(run + b) * c.Hkv + kv) * p.cols + col0 + n; };
+      for (int db = 0; db < DBN; ++db) part[l16 * (D / 4) + ((db * 4 + g4) ^ (l16 & SW))] = oacc[nc][db] * wscale;
       if (wr == 0 && lane < nh) {
         float sum = 0.f;
         for (int r = 0; r < NR; ++r) sum += l_s[w + r * WH][l16] * fast_exp2(m_s[w + r * WH][l16] - M_use);
         inv_s[w][l16] = sum > 0.f ? 1.f / sum : 0.f;
-        p.part_m[part_row(l16, hkv)] = sum > 0.f ? M_use + fast_log2(sum) : -INFINITY;
+        p.part_m[(piece + hkv) * p.cols + col0 + l16] = sum > 0.f ? M_use + fast_log2(sum) : -INFINITY;
       }
       __syncthreads();
-      for (int i = tid; i < WH * nh * D; i += NW * 64) {
-        const int d = i % D, n = i / D % nh, k = i / D / nh;
-        float o = 0.f;
-        for (int r = 0; r < NR; ++r) o += reinterpret_cast<const float*>(&vsm[k + r * WH][0])[n * D + d];
-        p.part_o[part_row(n, hgroup * WH + k) * D + d] = o * inv_s[k][n];
+      for (int k = 0; k < WH; ++k) {
+        for (int i = tid; i < nh * (D / 4); i += NW * 64) {
+          const int n = i / (D / 4), q = i % (D / 4);
+          f32x4 o = {0.f, 0.f, 0.f, 0.f};
+          for (int r = 0; r < NR; ++r)
+            o += reinterpret_cast<const f32x4*>(&vsm[k + r * WH][0])[n * (D / 4) + (q ^ (n & SW))];
+          *reinterpret_cast<f32x4*>(p.part_o + ((piece + hgroup * WH + k) * p.cols + col0 + n) * D + q * 4) = o * inv_s[k][n];
+        }
       }
       __syncthreads();   // before the ring and the statistics are written again
     }
@@ -792,13 +812,18 @@ __device__ void attend_alone(const PagedAttnParams& p, int b, int i, int h, cons
   }
 }
 
-// One wave per (token, query head): merge the pieces' partial outputs, sixteen per round trip.
+// One workgroup of four waves per (token, query head): merge the pieces' partial outputs.  Each
+// wave takes every fourth piece, eight of them in flight, with weights relative to its own
+// largest LSE, and the four sums meet in LDS in a fixed order.
 template <class T, bool FP8, int D>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(256)
 paged_combine_kernel(PagedAttnParams p) {
+  constexpr int DJ = (D + 63) / 64;
+  constexpr int CH = 8;
+  __shared__ float m_s[4], l_s[4], o_s[4][D];
   const PagedCache& c = p.c;
   const int h = blockIdx.x % c.Hq, t = blockIdx.x / c.Hq;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int b = 0, i = 0, ns = 0;
   const bool in = token_place(c, t, b, i);
   const bool alone = in && i >= c.n;   // past the stated longest sequence
@@ -811,10 +836,10 @@ paged_combine_kernel(PagedAttnParams p) {
       int sum;
       const int u = lane_units(c, at, p.unit_rows, lane, sum);
       if (b >= at && b < at + 64) {
-        mine = __shfl(u, b - at);
-        first = units + __shfl(sum, b - at) - mine;
+        mine = (int)lane_of((uint32_t)u, b - at);
+        first = units + (int)lane_of((uint32_t)sum, b - at) - mine;
       }
-      units += __shfl(sum, 63);
+      units += (int)lane_of((uint32_t)sum, 63);
     }
     if (mine > 0) {
       const Runs runs(units, p.parts);
@@ -824,19 +849,17 @@ paged_combine_kernel(PagedAttnParams p) {
     }
   }
   const int64_t row = (int64_t)t * c.Hq + h, step = (int64_t)c.Hkv * p.cols;
-  constexpr int DJ = (D + 63) / 64;
-  constexpr int CH = 16;
   float acc[DJ];
 #pragma unroll
   for (int j = 0; j < DJ; ++j) acc[j] = 0.f;
   float M = -INFINITY, wsum = 0.f;
-  for (int s0 = 0; s0 < ns; s0 += CH) {
+  for (int s0 = w; s0 < ns; s0 += 4 * CH) {
     float pm[CH], x[CH][DJ];
 #pragma unroll
     for (int u = 0; u < CH; ++u) {
-      const bool ok = s0 + u < ns;
-      pm[u] = ok ? p.part_m[base + (s0 + u) * step] : -INFINITY;
-      const float* po = p.part_o + (base + (s0 + u) * step) * D;
+      const bool ok = s0 + 4 * u < ns;
+      pm[u] = ok ? p.part_m[base + (s0 + 4 * u) * step] : -INFINITY;
+      const float* po = p.part_o + (base + (s0 + 4 * u) * step) * D;
 #pragma unroll
       for (int j = 0; j < DJ; ++j) x[u][j] = (ok && lane + 64 * j < D) ? po[lane + 64 * j] : 0.f;
     }
@@ -858,29 +881,40 @@ paged_combine_kernel(PagedAttnParams p) {
     }
     M = Mn;
   }
-  if (alone)
+  if (alone && w == 0)
     attend_alone<T, FP8, D>(p, b, i, h, (const T*)p.q + t * p.q_ss + h * p.q_sh, acc, M, wsum);
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
-  T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
+  if (lane == 0) m_s[w] = M, l_s[w] = wsum;
 #pragma unroll
-  for (int j = 0; j < DJ; ++j) {
-    const int d = lane + 64 * j;
-    if (d < D) orow[d] = (T)(acc[j] * inv);
+  for (int j = 0; j < DJ; ++j)
+    if (lane + 64 * j < D) o_s[w][lane + 64 * j] = acc[j];
+  __syncthreads();
+  const float top = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
+  float f[4], sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    f[u] = m_s[u] == -INFINITY ? 0.f : fast_exp2(m_s[u] - top);
+    sum += l_s[u] * f[u];
   }
-  if (p.lse && lane == 0) p.lse[row] = wsum > 0.f ? (M + fast_log2(wsum)) * kLn2 : -INFINITY;
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
+  for (int d = threadIdx.x; d < D; d += 256)
+    orow[d] = (T)((o_s[0][d] * f[0] + o_s[1][d] * f[1] + o_s[2][d] * f[2] + o_s[3][d] * f[3]) * inv);
+  if (p.lse && threadIdx.x == 0) p.lse[row] = sum > 0.f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
 }
 
 #ifndef FAL_PAGED_PIECE
 #define FAL_PAGED_PIECE 512
 #endif
 #ifndef FAL_PAGED_WPC
-#define FAL_PAGED_WPC 3
+#define FAL_PAGED_WPC 1
 #endif
 #ifndef FAL_PAGED_UNIT
 #define FAL_PAGED_UNIT 64
 #endif
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, int row_bytes, int ncu) {
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, int row_bytes,
+                     int ncu) {
   PagedPlan r{};
+  const int waves = paged_waves(d, fp8);
   const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
   r.nc = cols <= 16 || d > 128 ? 1 : 2;   // (head dim 256: two tiles would not fit the registers)
   r.col_tiles = (int)((cols + 16 * r.nc - 1) / (16 * r.nc));
@@ -888,7 +922,7 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t
   r.wave_heads = 1;
   while (r.wave_heads < 4 && Hkv % (2 * r.wave_heads) == 0 && row_bytes * r.wave_heads < FAL_PAGED_PIECE) r.wave_heads *= 2;
   // a unit: two steps, which are in flight together, for each wave
-  r.unit_rows = FAL_PAGED_UNIT * kPagedWaves / r.wave_heads;
+  r.unit_rows = FAL_PAGED_UNIT * waves / r.wave_heads;
   const int64_t most = B * ((capacity + r.unit_rows - 1) / r.unit_rows);
   int64_t parts = (int64_t)ncu * FAL_PAGED_WPC / (Hkv / r.wave_heads * r.col_tiles);
   parts = parts < 1 ? 1 : parts > most ? most : parts;
@@ -898,12 +932,12 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t
 
 template <class T, bool FP8, int D>
 static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.parts * (p.c.Hkv / p.wave_heads) * p.col_tiles)), block(kPagedWaves * 64);
+  const dim3 grid((unsigned)(p.parts * (p.c.Hkv / p.wave_heads) * p.col_tiles)), block(paged_waves(D, FP8) * 64);
   if (D > 128 || p.nc == 1) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((paged_split_kernel<T, FP8, (D > 128 ? 128 : D), 2>), grid, block, 0, st, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(64), 0, st, p);
+  hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
