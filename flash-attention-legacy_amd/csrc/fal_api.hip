@@ -961,7 +961,7 @@ PagedPlan plan_of(const fal_paged_cache& c) {
   // bytes that a head's row has for itself: a whole page where heads lie one after the other
   const bool by_row = c.heads_kv > 1 && c.k_strides[1] < c.k_strides[2];
   const int64_t row_bytes = (c.fp8 ? 1 : 2) * c.head_dim * (by_row ? 1 : c.page_size);
-  return paged_plan(c.batch, c.seqlen, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim, c.fp8 != 0,
+  return paged_plan(c.batch, c.seqlen, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim, c.fp8 != 0, c.cu_seqlens != nullptr,
                     (int)std::min<int64_t>(row_bytes, 1 << 20), std::max(device_cu_count(), 1));
 }
 
@@ -986,7 +986,7 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   p.causal = is_causal != 0;
   const PagedPlan plan = plan_of(c);
   p.parts = plan.parts, p.unit_rows = plan.unit_rows, p.wave_heads = plan.wave_heads;
-  p.nc = plan.nc, p.col_tiles = plan.col_tiles, p.cols = plan.cols;
+  p.nc = plan.nc, p.col_tiles = plan.col_tiles, p.cols = plan.cols, p.direct = plan.direct;
   const size_t rows = (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
   p.part_o = static_cast<float*>(workspace);
   p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(rows * c.head_dim * sizeof(float)));
@@ -1025,6 +1025,7 @@ size_t fal_paged_attn_workspace_size(const fal_paged_cache* cache) {
       !dims_ok(c.total_tokens) || c.page_size <= 0 || c.max_pages < 0 || c.max_pages > (1 << 30) / c.page_size)
     return 0;
   const PagedPlan plan = plan_of(c);
+  if (plan.direct) return 0;
   const size_t rows = (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
   return align256(rows * c.head_dim * sizeof(float)) + align256(rows * sizeof(float));
 }

@@ -185,13 +185,14 @@ struct PagedAttnParams {
   int negate_q;
   int causal;
   // split kernel: the sequences' rows, in units of unit_rows, in `parts` equal runs; one workgroup
-  // per (run, wave_heads KV heads, nc tiles of 16 columns)
-  int parts, unit_rows, wave_heads, nc, col_tiles, cols;
+  // per (run, wave_heads KV heads, nc tiles of 16 columns); direct: a run is a sequence, and there
+  // is nothing to merge
+  int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
   float* part_o;      // [parts + B, Hkv, cols, d]
   float* part_m;      // [parts + B, Hkv, cols] log2-domain LSE
 };
 struct PagedPlan {
-  int parts, unit_rows, wave_heads, nc, col_tiles, cols;
+  int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
 };
 
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);
@@ -258,7 +259,7 @@ hipError_t launch_decode(const DecodeParams& p, int d, hipStream_t st);
 hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st);
 hipError_t launch_paged_attn(const PagedAttnParams& p, int d, hipStream_t st);
 // row_bytes: bytes next to each other that belong to one KV head
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8,
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
                      int row_bytes, int ncu);
 
 }  // namespace fal

@@ -431,9 +431,13 @@ __device__ __forceinline__ int lanes_scan(int x) {
   return x;
 }
 
-// Units of 64 sequences, one per lane, and their inclusive sums.
+// Units of 64 sequences, one per lane, and their inclusive sums.  The first unit of a sequence
+// has no rows: it stands for what starting and ending one costs (page table, scales, first rows,
+// merge: about as long as UNITUS of streaming), so that runs that cross into the next sequence
+// get fewer rows and all end together.
 __device__ __forceinline__ int lane_units(const PagedCache& c, int base, int unit_rows, int lane, int& sum) {
-  const int u = base + lane < c.B ? cdiv(cache_rows(c, base + lane), unit_rows) : 0;
+  const int rows = base + lane < c.B ? cache_rows(c, base + lane) : 0;
+  const int u = rows > 0 ? cdiv(rows, unit_rows) + 1 : 0;
   sum = lanes_scan(u);
   return u;
 }
@@ -447,7 +451,10 @@ paged_split_kernel(PagedAttnParams p) {
   using VS = VSlice<FP8, D>;
   // K registers of a slice: 16-byte pieces that cover 64 bytes of each of its 16 rows
   constexpr int KL = FP8 ? D / 64 : D / 32, KTAIL = FP8 ? (D % 64) / 32 : 0;   // (tail: 32 bytes of each row)
-  constexpr bool LINE = KL >= 2;                 // pairs of pieces loaded as whole 128-byte lines
+#ifndef FAL_PAGED_LINE
+#define FAL_PAGED_LINE 1
+#endif
+  constexpr bool LINE = KL >= 2 && FAL_PAGED_LINE;   // pairs of pieces loaded as whole 128-byte lines
   constexpr int LPS = 2 * (KL + KTAIL + VS::LOADS);
   using V8 = vec8<T>;
   __shared__ __attribute__((aligned(1024))) uint8_t vsm[NW][4 * VS::BYTES];   // 2 steps x 2 slices
@@ -473,7 +480,9 @@ paged_split_kernel(PagedAttnParams p) {
 
   // this run's first sequence and unit
   int b = 0, local = 0, left;
-  {
+  if (p.direct) {        // one run is one sequence
+    b = run, left = 0x7fffffff;
+  } else {
     int sum, u = 0;
     int64_t units = 0;
     for (int base = 0; base < c.B; base += 64) {
@@ -527,14 +536,16 @@ paged_split_kernel(PagedAttnParams p) {
 
   for (; left > 0; ++b, local = 0) {
     const int L = cache_rows(c, b);
-    const int take = min(left, cdiv(L, p.unit_rows) - local);
-    left -= take;
-    const int row0 = local * p.unit_rows, row1 = min(L, (local + take) * p.unit_rows);
+    const int take = min(left, (L > 0 ? cdiv(L, p.unit_rows) + 1 : 0) - local);
+    left = p.direct ? 0 : left - take;
+    const int row0 = max(local - 1, 0) * p.unit_rows, row1 = min(L, (local + take - 1) * p.unit_rows);
     int off, len;
     token_range(c, b, off, len);
     const int ncols = min(len, c.n) * G;
-    if (row0 >= row1 || ct * NC * 16 >= ncols) continue;
+    if ((row0 >= row1 && !p.direct) || ct * NC * 16 >= ncols) continue;
 
+    // rows below this one are seen by every column
+    const int lim_first = p.causal ? L - len + ct * NC * 16 / G + 1 : L;
     // queries of the columns as the B operand (n = column, k = head dim in K's order)
     V8 qreg[NC][KS];
     int lim[NC];         // rows below this one are seen by the column
@@ -644,47 +655,53 @@ paged_split_kernel(PagedAttnParams p) {
         }
       }
       const int n0 = (int)lane_of((uint32_t)nrow, 2 * jj), n1 = (int)lane_of((uint32_t)nrow, 2 * jj + 1);
+      // scores stay unscaled until their exponent: max and mask commute with a positive factor
       float kfac[2] = {p.scale_log2, p.scale_log2};
       if constexpr (FP8) {
-        kfac[0] *= lane_of(ksc, 2 * jj), kfac[1] *= lane_of(ksc, 2 * jj + 1);
+        kfac[0] = fmaxf(kfac[0] * lane_of(ksc, 2 * jj), 0x1p-126f), kfac[1] = fmaxf(kfac[1] * lane_of(ksc, 2 * jj + 1), 0x1p-126f);
         const float v0 = n0 > 0 ? lane_of(vsc, 2 * jj) : 0.f, v1 = n1 > 0 ? lane_of(vsc, 2 * jj + 1) : 0.f;
         const float now = fmaxf(ref, fmaxf(v0, v1));
         const float inv = now >= 0x1p-126f ? __builtin_amdgcn_rcpf(now) : 0.f;
         vfac[0] = v0 * inv, vfac[1] = v1 * inv, back = ref * inv;
         ref = now;
       }
+      const int r0 = k_begin + j * 32;
+      const bool whole = n0 == 16 && n1 == 16 && r0 + 32 <= lim_first;   // every row seen by every column
       V8 pb[NC];
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
-        const int r0 = k_begin + j * 32 + 4 * g4;
-        float mx = -INFINITY;
+        if (!whole) {
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl)
+          for (int sl = 0; sl < 2; ++sl)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool seen = 4 * g4 + i < (sl ? n1 : n0) && r0 + sl * 16 + i < lim[nc];
-            const float x = seen ? s[nc][sl][i] * kfac[sl] : -INFINITY;
-            s[nc][sl][i] = x;
-            mx = fmaxf(mx, x);
-          }
+            for (int i = 0; i < 4; ++i) {
+              const int r = 4 * g4 + i;
+              if (r >= (sl ? n1 : n0) || r0 + sl * 16 + r >= lim[nc]) s[nc][sl][i] = -INFINITY;
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[nc][0][0], s[nc][0][1]), fmaxf(s[nc][0][2], s[nc][0][3])) * kfac[0],
+                         fmaxf(fmaxf(s[nc][1][0], s[nc][1][1]), fmaxf(s[nc][1][2], s[nc][1][3])) * kfac[1]);
         mx = quarters_max(mx);
         const float m_new = fmaxf(m_run[nc], mx);
         const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
-        const float alpha = fast_exp2(m_run[nc] - m_use);
-        m_run[nc] = m_new;
-        float l = l_run[nc] * alpha;
+        float l = 0.f;
 #pragma unroll
         for (int sl = 0; sl < 2; ++sl)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e = fast_exp2(s[nc][sl][i] - m_use);
+            const float e = fast_exp2(fmaf(s[nc][sl][i], kfac[sl], -m_use));
             l += e;
             pb[nc][sl * 4 + i] = (T)(FP8 ? e * vfac[sl] : e);
           }
-        l_run[nc] = l;
-        const float f = FP8 ? alpha * back : alpha;
+        if (__any(m_new != m_run[nc]) || (FP8 && back != 1.f)) {
+          const float alpha = fast_exp2(m_run[nc] - m_use);
+          l_run[nc] *= alpha;
+          m_run[nc] = m_new;
+          const float f = FP8 ? alpha * back : alpha;
 #pragma unroll
-        for (int db = 0; db < DBN; ++db) oacc[nc][db] *= f;
+          for (int db = 0; db < DBN; ++db) oacc[nc][db] *= f;
+        }
+        l_run[nc] += l;
       }
       // O^T += V^T P^T over the 32 rows
 #pragma unroll
@@ -713,8 +730,20 @@ paged_split_kernel(PagedAttnParams p) {
     }
     }
 
-    // ---- the piece's partial output, normalised, and its log2-domain LSE ----
+    // ---- the piece's partial output, normalised, and its log2-domain LSE; or the result ----
     const int64_t piece = (int64_t)(run + b) * c.Hkv;
+    auto put = [&](int col, int kv, int d, f32x4 x) {
+      if (!p.direct) {
+        *reinterpret_cast<f32x4*>(p.part_o + ((piece + kv) * p.cols + col) * D + d) = x;
+        return;
+      }
+      const vec4<T> y = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+      *reinterpret_cast<vec4<T>*>((T*)p.o + b * p.o_sb + col / G * p.o_ss + (kv * G + col % G) * p.o_sh + d) = y;
+    };
+    auto put_lse = [&](int col, int kv, float lse2) {
+      if (!p.direct) p.part_m[(piece + kv) * p.cols + col] = lse2;
+      else if (p.lse) p.lse[((int64_t)b * c.n + col / G) * c.Hq + kv * G + col % G] = lse2 * kLn2;
+    };
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       const int col0 = (ct * NC + nc) * 16;
@@ -722,12 +751,10 @@ paged_split_kernel(PagedAttnParams p) {
       const float l_tot = quarters_sum(l_run[nc]);
       if (NR == 1) {   // a wave has all of its head's rows
         const float f = l_tot > 0.f ? (FP8 ? ref : 1.f) / l_tot : 0.f;
-        const int64_t row = (piece + hkv) * p.cols + col0 + l16;
         if (l16 < nh) {
 #pragma unroll
-          for (int db = 0; db < DBN; ++db)
-            *reinterpret_cast<f32x4*>(p.part_o + row * D + db * 16 + 4 * g4) = oacc[nc][db] * f;
-          if (g4 == 0) p.part_m[row] = l_tot > 0.f ? m_run[nc] + fast_log2(l_tot) : -INFINITY;
+          for (int db = 0; db < DBN; ++db) put(col0 + l16, hkv, db * 16 + 4 * g4, oacc[nc][db] * f);
+          if (g4 == 0) put_lse(col0 + l16, hkv, l_tot > 0.f ? m_run[nc] + fast_log2(l_tot) : -INFINITY);
         }
         continue;
       }
@@ -737,8 +764,11 @@ paged_split_kernel(PagedAttnParams p) {
         l_s[w][l16] = l_tot;
       }
       __syncthreads();
-      float M = -INFINITY;
-      for (int r = 0; r < NR; ++r) M = fmaxf(M, m_s[ws % WH + r * WH][l16]);
+      float M = -INFINITY, mw[NW], lw[NW];   // (of all waves: the reads then go out together)
+#pragma unroll
+      for (int i = 0; i < NW; ++i) mw[i] = m_s[i][l16], lw[i] = l_s[i][l16];
+#pragma unroll
+      for (int i = 0; i < NW; ++i) M = i % WH == ws % WH ? fmaxf(M, mw[i]) : M;
       const float M_use = (M == -INFINITY) ? 0.f : M;
       const float wscale = fast_exp2(m_run[nc] - M_use) * (FP8 ? ref : 1.f);
       constexpr int SW = D / 4 >= 16 && D != 96 ? 15 : 7;
@@ -747,18 +777,20 @@ paged_split_kernel(PagedAttnParams p) {
       for (int db = 0; db < DBN; ++db) part[l16 * (D / 4) + ((db * 4 + g4) ^ (l16 & SW))] = oacc[nc][db] * wscale;
       if (wr == 0 && lane < nh) {
         float sum = 0.f;
-        for (int r = 0; r < NR; ++r) sum += l_s[w + r * WH][l16] * fast_exp2(m_s[w + r * WH][l16] - M_use);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) sum += i % WH == ws % WH ? lw[i] * fast_exp2(mw[i] - M_use) : 0.f;
         inv_s[w][l16] = sum > 0.f ? 1.f / sum : 0.f;
-        p.part_m[(piece + hkv) * p.cols + col0 + l16] = sum > 0.f ? M_use + fast_log2(sum) : -INFINITY;
+        put_lse(col0 + l16, hkv, sum > 0.f ? M_use + fast_log2(sum) : -INFINITY);
       }
       __syncthreads();
       for (int k = 0; k < WH; ++k) {
         for (int i = tid; i < nh * (D / 4); i += NW * 64) {
           const int n = i / (D / 4), q = i % (D / 4);
           f32x4 o = {0.f, 0.f, 0.f, 0.f};
-          for (int r = 0; r < NR; ++r)
-            o += reinterpret_cast<const f32x4*>(&vsm[k + r * WH][0])[n * (D / 4) + (q ^ (n & SW))];
-          *reinterpret_cast<f32x4*>(p.part_o + ((piece + hgroup * WH + k) * p.cols + col0 + n) * D + q * 4) = o * inv_s[k][n];
+#pragma unroll
+          for (int r = 0; r < NW; ++r)
+            if (r < NR) o += reinterpret_cast<const f32x4*>(&vsm[k + r * WH][0])[n * (D / 4) + (q ^ (n & SW))];
+          put(col0 + n, hgroup * WH + k, q * 4, o * inv_s[k][n]);
         }
       }
       __syncthreads();   // before the ring and the statistics are written again
@@ -843,7 +875,8 @@ paged_combine_kernel(PagedAttnParams p) {
     }
     if (mine > 0) {
       const Runs runs(units, p.parts);
-      const int g0 = runs.of(first);
+      int g0 = runs.of(first);
+      if (runs.begin(g0 + 1) == first + 1) ++g0;   // (nothing but the unit without rows)
       ns = runs.of(first + mine - 1) - g0 + 1;
       base = ((int64_t)(g0 + b) * c.Hkv + h / G) * p.cols + i * G + h % G;
     }
@@ -902,17 +935,20 @@ paged_combine_kernel(PagedAttnParams p) {
   if (p.lse && threadIdx.x == 0) p.lse[row] = sum > 0.f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
 }
 
-#ifndef FAL_PAGED_PIECE
-#define FAL_PAGED_PIECE 512
+#ifndef FAL_PAGED_WH
+#define FAL_PAGED_WH 4
 #endif
 #ifndef FAL_PAGED_WPC
 #define FAL_PAGED_WPC 1
 #endif
 #ifndef FAL_PAGED_UNIT
-#define FAL_PAGED_UNIT 64
+#define FAL_PAGED_UNIT 32
 #endif
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, int row_bytes,
-                     int ncu) {
+#ifndef FAL_PAGED_DIRECT
+#define FAL_PAGED_DIRECT 2048
+#endif
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
+                     int row_bytes, int ncu) {
   PagedPlan r{};
   const int waves = paged_waves(d, fp8);
   const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
@@ -920,13 +956,13 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t
   r.col_tiles = (int)((cols + 16 * r.nc - 1) / (16 * r.nc));
   r.cols = r.col_tiles * 16 * r.nc;
   r.wave_heads = 1;
-  while (r.wave_heads < 4 && Hkv % (2 * r.wave_heads) == 0 && row_bytes * r.wave_heads < FAL_PAGED_PIECE) r.wave_heads *= 2;
-  // a unit: two steps, which are in flight together, for each wave
+  r.direct = capacity <= FAL_PAGED_DIRECT && !packed;
+  while (!r.direct && r.wave_heads < FAL_PAGED_WH && Hkv % (2 * r.wave_heads) == 0) r.wave_heads *= 2;
   r.unit_rows = FAL_PAGED_UNIT * waves / r.wave_heads;
-  const int64_t most = B * ((capacity + r.unit_rows - 1) / r.unit_rows);
+  const int64_t most = B * ((capacity + r.unit_rows - 1) / r.unit_rows + 1);
   int64_t parts = (int64_t)ncu * FAL_PAGED_WPC / (Hkv / r.wave_heads * r.col_tiles);
   parts = parts < 1 ? 1 : parts > most ? most : parts;
-  r.parts = (int)(parts < 1 ? 1 : parts);
+  r.parts = (int)(r.direct ? B : parts < 1 ? 1 : parts);
   return r;
 }
 
@@ -936,7 +972,7 @@ static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
   if (D > 128 || p.nc == 1) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((paged_split_kernel<T, FP8, (D > 128 ? 128 : D), 2>), grid, block, 0, st, p);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || p.direct) return e;
   hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
