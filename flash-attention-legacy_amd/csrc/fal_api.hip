@@ -957,6 +957,12 @@ int paged_append_impl(const fal_paged_cache* cache, const void* k, const void* v
   return launch_status(launch_paged_append(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_append");
 }
 
+// Rows of partial outputs in the workspace
+size_t paged_partials(const PagedPlan& plan, const fal_paged_cache& c) {
+  if (plan.splits) return plan.splits > 1 ? (size_t)c.total_tokens * c.heads_q * plan.splits : 0;
+  return plan.direct ? 0 : (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
+}
+
 PagedPlan plan_of(const fal_paged_cache& c) {
   // bytes that a head's row has for itself: a whole page where heads lie one after the other
   const bool by_row = c.heads_kv > 1 && c.k_strides[1] < c.k_strides[2];
@@ -987,12 +993,19 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   const PagedPlan plan = plan_of(c);
   p.parts = plan.parts, p.unit_rows = plan.unit_rows, p.wave_heads = plan.wave_heads;
   p.nc = plan.nc, p.col_tiles = plan.col_tiles, p.cols = plan.cols, p.direct = plan.direct;
-  const size_t rows = (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
+  p.splits = plan.splits, p.tile_cols = plan.tile_cols;
+  const size_t rows = paged_partials(plan, c);
   p.part_o = static_cast<float*>(workspace);
   p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(rows * c.head_dim * sizeof(float)));
-  if (c.total_tokens * c.heads_q > 0x7fffffff || c.seqlen * c.heads_q > 0x7fffffff ||
-      (int64_t)plan.parts * c.heads_kv * plan.col_tiles > 0x7fffffff ||
-      c.batch * ((c.max_pages * c.page_size + plan.unit_rows - 1) / plan.unit_rows) / plan.parts >= 0x7fffffff)
+  if (c.total_tokens * c.heads_q > 0x7fffffff || c.seqlen * c.heads_q > 0x7fffffff)
+    return fail(FAL_ERR_INVALID, "problem too large for one launch");
+  if (plan.splits) {
+    const int64_t per = (int64_t)plan.splits * c.heads_kv * plan.tile_cols;
+    if (c.batch > (0x7fffffff - 64) / per) return fail(FAL_ERR_INVALID, "problem too large for one launch");
+    p.tile_blocks = (int)(c.batch * per);
+    p.rest_blocks = c.cu_seqlens ? 16 : 0;
+  } else if ((int64_t)plan.parts * c.heads_kv * plan.col_tiles > 0x7fffffff ||
+             c.batch * ((c.max_pages * c.page_size + plan.unit_rows - 1) / plan.unit_rows + 1) / plan.parts >= 0x7fffffff)
     return fail(FAL_ERR_INVALID, "problem too large for one launch");
   return launch_status(launch_paged_attn(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_attn");
 }
@@ -1025,8 +1038,8 @@ size_t fal_paged_attn_workspace_size(const fal_paged_cache* cache) {
       !dims_ok(c.total_tokens) || c.page_size <= 0 || c.max_pages < 0 || c.max_pages > (1 << 30) / c.page_size)
     return 0;
   const PagedPlan plan = plan_of(c);
-  if (plan.direct) return 0;
-  const size_t rows = (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
+  const size_t rows = paged_partials(plan, c);
+  if (!rows) return 0;
   return align256(rows * c.head_dim * sizeof(float)) + align256(rows * sizeof(float));
 }
 int fal_paged_attn(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,

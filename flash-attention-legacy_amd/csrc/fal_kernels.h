@@ -188,11 +188,15 @@ struct PagedAttnParams {
   // per (run, wave_heads KV heads, nc tiles of 16 columns); direct: a run is a sequence, and there
   // is nothing to merge
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
-  float* part_o;      // [parts + B, Hkv, cols, d]
-  float* part_m;      // [parts + B, Hkv, cols] log2-domain LSE
+  // tile kernel (splits > 0): tile_cols column tiles of the longest sequence, each sequence's rows
+  // in `splits` shares; tile_blocks workgroups, and rest_blocks for packed rows outside every sequence
+  int splits, tile_cols, tile_blocks, rest_blocks;
+  float* part_o;      // [parts + B, Hkv, cols, d], or [total, Hq, splits, d]
+  float* part_m;      // the same without d: log2-domain LSE
 };
 struct PagedPlan {
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
+  int splits, tile_cols, max_cols;
 };
 
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);

@@ -798,6 +798,273 @@ paged_split_kernel(PagedAttnParams p) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Attention, many columns: tiles of keys shared by a workgroup
+// ---------------------------------------------------------------------------
+// One workgroup takes 128 columns (see above) of one sequence and KV head, 32 to a wave, and
+// walks tiles of 64 rows; with few workgroups, `splits` of them share a column tile's rows.
+// * Wave w brings the tile's slice w (16 rows of one page) from the cache: its page and scales
+//   are scalars, its lanes' places in the page constants, and e4m3 codes become 16-bit values
+//   once, on the way to LDS, not once per wave that reads them.  Loads of a tile run a whole
+//   tile ahead, its page number two.
+// * S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMA; the S^T accumulators are P^T's operand in
+//   place (fal_common.h).
+// * The running maximum that exponents are taken from moves only when a score passes it by 8:
+//   P reaches 2^8 at most, and the accumulators are rarely rescaled.
+// * Scales as in the split kernel: the value factor enters the exponent, and each slice's sum is
+//   divided by it again for l.
+constexpr int kTileRows = 64, kTileCols = 128;
+
+template <class T, bool FP8, int D>
+__global__ void __launch_bounds__(256, D > 128 ? 1 : 2)
+paged_tile_kernel(PagedAttnParams p) {
+  constexpr int DB = D / 32, KS = D / 16;
+  constexpr int RB = FP8 ? D : 2 * D, CPR = RB / 16;         // bytes of a cache row, its 16-byte pieces
+  constexpr int LOADS = (16 * CPR + 63) / 64;                // pieces per lane of a slice
+  constexpr int CB = FP8 ? 1 : 2;
+  using V8 = vec8<T>;
+  using Tile = SwizzledTile<D>;
+  __shared__ __attribute__((aligned(1024))) T ksm[2][kTileRows * D], vsm[2][kTileRows * D];
+  __shared__ float ssm[2][4][2];                             // per slice: key and value scale (-1: no page)
+
+  const PagedCache& c = p.c;
+  const int G = c.Hq / c.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if ((int)blockIdx.x >= p.tile_blocks) {   // packed rows outside every sequence
+    const int lo = min(max(c.cu[0], 0), c.total), hi = max(min(max(c.cu[c.B], 0), c.total), lo);
+    for (int64_t r = ((int)blockIdx.x - p.tile_blocks) * 4 + w; r < (int64_t)(lo + c.total - hi) * c.Hq; r += 4 * p.rest_blocks) {
+      const int64_t t = r / c.Hq < lo ? r / c.Hq : r / c.Hq - lo + hi;
+      const int h = (int)(r % c.Hq);
+      for (int d = lane; d < D; d += 64) ((T*)p.o + t * p.o_ss + h * p.o_sh)[d] = (T)0.f;
+      if (p.lse && lane == 0) p.lse[t * c.Hq + h] = -INFINITY;
+    }
+    return;
+  }
+  int rest = blockIdx.x;
+  const int hkv = rest % c.Hkv;
+  rest /= c.Hkv;
+  const int b = rest % c.B;
+  rest /= c.B;
+  const int split = rest % p.splits;
+  int off, len;
+  token_range(c, b, off, len);
+  const int L = cache_rows(c, b), ncols = len * G;
+  // column tiles, those that see the most rows first; past the stated longest sequence each
+  // workgroup takes further ones
+  for (int ct = p.tile_cols - 1 - rest / p.splits; ct * kTileCols < ncols; ct += p.tile_cols) {
+    const int col_last = min(ncols, (ct + 1) * kTileCols) - 1;
+    const int k_hi = max(p.causal ? L - len + col_last / G + 1 : L, 0);
+    const int tiles = cdiv(k_hi, kTileRows);
+    const int t0 = (int)((int64_t)tiles * split / p.splits), t1 = (int)((int64_t)tiles * (split + 1) / p.splits);
+
+    // this wave's columns
+    const int col = ct * kTileCols + w * 32 + l32, i_tok = col / G, head = hkv * G + col % G;
+    const bool have = col < ncols, active = ct * kTileCols + w * 32 < ncols;
+    const int lim = p.causal ? L - len + i_tok + 1 : L;
+    const int lim_first = p.causal ? L - len + (ct * kTileCols + w * 32) / G + 1 : L;
+    V8 qreg[KS];
+    const T* qrow = (const T*)p.q + (c.cu ? (int64_t)(off + i_tok) * p.q_ss : b * p.q_sb + i_tok * p.q_ss) + head * p.q_sh;
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      qreg[t] = have ? ld8(qrow + t * 16 + hh * 8) : zero8<T>();
+      if (p.negate_q) qreg[t] = -qreg[t];
+    }
+    f32x16 oacc[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) oacc[i] = zero_f16();
+    float m_ref = -INFINITY, l_run = 0.f, ref = 0.f;
+
+    // staging: this lane's pieces of the wave's slice
+    const int k_ss = (int)c.k_ss * CB, v_ss = (int)c.v_ss * CB;
+    int kv[LOADS], vv[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int e = i * 64 + lane, r = e / CPR, u = e % CPR;
+      kv[i] = r < 16 ? r * k_ss + u * 16 : 0x7ffffff0;
+      vv[i] = r < 16 ? r * v_ss + u * 16 : 0x7ffffff0;
+    }
+    auto page_of = [&](int tile) {   // page number of this wave's slice, -1: none
+      const int r = tile * kTileRows + w * 16;
+      if (tile >= t1 || r >= k_hi) return -1;
+      const int pid = c.table[b * c.table_sb + r / c.page_size];
+      return pid >= 0 && pid < c.num_pages ? pid : -1;
+    };
+    u32x4 kreg[LOADS], vreg[LOADS];
+    float ksc = 1.f, vsc = 1.f;
+    auto fetch = [&](int tile, int pid) {
+      const int r = tile * kTileRows + w * 16, slot = r % c.page_size;
+      const int n = pid >= 0 ? min(16, k_hi - r) : 0;
+      const int64_t at = pid >= 0 ? pid : 0;
+      const auto krs = make_rsrc((const char*)c.k + (at * c.k_sp + hkv * c.k_sh + slot * c.k_ss) * CB,
+                                 n > 0 ? (uint32_t)((n - 1) * k_ss + RB) : 0);
+      const auto vrs = make_rsrc((const char*)c.v + (at * c.v_sp + hkv * c.v_sh + slot * c.v_ss) * CB,
+                                 n > 0 ? (uint32_t)((n - 1) * v_ss + RB) : 0);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        kreg[i] = __builtin_amdgcn_raw_buffer_load_b128(krs, kv[i], 0, 0);
+        vreg[i] = __builtin_amdgcn_raw_buffer_load_b128(vrs, vv[i], 0, 0);
+      }
+      if (FP8 && n > 0) {
+        ksc = c.k_scale[pid * c.ks_sp + hkv * c.ks_sh];
+        vsc = c.v_scale[pid * c.vs_sp + hkv * c.vs_sh];
+      }
+      if (n <= 0) vsc = -1.f;
+      else if (!FP8) vsc = 1.f;
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = i * 64 + lane, r = e / CPR, u = e % CPR, row = w * 16 + r;
+        if (16 * CPR % 64 != 0 && r >= 16) continue;
+        if constexpr (FP8) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            st_u4(&ksm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(kreg[i][2 * x], kreg[i][2 * x + 1])));
+            st_u4(&vsm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(vreg[i][2 * x], vreg[i][2 * x + 1])));
+          }
+        } else {
+          st_u4(&ksm[buf][Tile::offset(row, u)], kreg[i]);
+          st_u4(&vsm[buf][Tile::offset(row, u)], vreg[i]);
+        }
+      }
+      if (lane == 0) ssm[buf][w][0] = ksc, ssm[buf][w][1] = vsc;
+    };
+
+    if (t0 < t1) {
+      int pid = page_of(t0 + 1);
+      fetch(t0, page_of(t0));
+      stage(0);
+      fetch(t0 + 1, pid);
+      pid = page_of(t0 + 2);
+      __syncthreads();
+      for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        if (active) {
+          // S^T: element i of block mb is row mb * 32 + (i / 4) * 8 + hh * 4 + i % 4, column l32
+          f32x16 s[2];
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb) {
+            s[mb] = zero_f16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+              s[mb] = mfma32(ld8(&ksm[buf][Tile::offset(mb * 32 + l32, ks * 2 + hh)]), qreg[ks], s[mb]);
+          }
+          // slice x: elements 8 (x % 2) .. + 8 of block x / 2
+          float kfac[4], vlog[4], vinv[4], back = 1.f;
+          bool whole = (t + 1) * kTileRows <= lim_first;
+          if constexpr (FP8) {
+            float v[4], now = ref;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              kfac[x] = fmaxf(p.scale_log2 * ssm[buf][x][0], 0x1p-126f);
+              v[x] = ssm[buf][x][1];
+              whole = whole && __builtin_amdgcn_readfirstlane(__float_as_int(v[x])) >= 0;
+              now = fmaxf(now, v[x]);
+            }
+            const float inv = now >= 0x1p-126f ? __builtin_amdgcn_rcpf(now) : 0.f;
+            back = ref * inv;
+            ref = now;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {   // (a value scale 2^60 below the largest counts as that)
+              const float f = fmaxf(v[x] * inv, 0x1p-60f);
+              vlog[x] = fast_log2(f), vinv[x] = __builtin_amdgcn_rcpf(f);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              kfac[x] = p.scale_log2, vlog[x] = 0.f, vinv[x] = 1.f;
+              whole = whole && __builtin_amdgcn_readfirstlane(__float_as_int(ssm[buf][x][1])) >= 0;
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const bool none = ssm[buf][x][1] < 0.f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = t * kTileRows + x * 16 + (i / 4) * 8 + hh * 4 + i % 4;
+                if (none || r >= lim) s[x / 2][(x & 1) * 8 + i] = -INFINITY;
+              }
+            }
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const f32x16& y = s[x / 2];
+            const int o = (x & 1) * 8;
+            const float a = fmaxf(fmaxf(fmaxf(y[o], y[o + 1]), fmaxf(y[o + 2], y[o + 3])),
+                                  fmaxf(fmaxf(y[o + 4], y[o + 5]), fmaxf(y[o + 6], y[o + 7])));
+            mx = fmaxf(mx, a * kfac[x]);
+          }
+          mx = pair_max(mx);
+          if (__any(mx > m_ref + 8.f) || (FP8 && back != 1.f)) {
+            const float m_new = mx > m_ref ? mx : m_ref;
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
+            m_ref = m_new;
+            l_run *= alpha;
+            const float f = alpha * back;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) oacc[i] *= f;
+          }
+          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+          V8 pb[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float sub = FP8 ? vlog[x] - m_use : -m_use;
+            float l = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float e = fast_exp2(fmaf(s[x / 2][(x & 1) * 8 + i], kfac[x], sub));
+              l += e;
+              pb[x][i] = (T)e;
+            }
+            l_run = FP8 ? fmaf(l, vinv[x], l_run) : l_run + l;
+          }
+          // O^T += V^T P^T
+          const int tr = hh * 4 + ((lane & 15) >> 2), tc = ((lane & 16) >> 3) + ((lane & 3) >> 1);
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const V8 a = join8(lds_tr(&vsm[buf][Tile::offset(x * 16 + tr, db * 4 + tc) + (lane & 1) * 4]),
+                                 lds_tr(&vsm[buf][Tile::offset(x * 16 + 8 + tr, db * 4 + tc) + (lane & 1) * 4]));
+              oacc[db] = mfma32(a, pb[x], oacc[db]);
+            }
+        }
+        if (t + 1 < t1) {
+          stage(buf ^ 1);
+          fetch(t + 2, pid);
+          pid = page_of(t + 3);
+        }
+        __syncthreads();
+      }
+    }
+
+    if (have) {
+      l_run = pair_sum(l_run);
+      const float f = l_run > 0.f ? (FP8 ? ref : 1.f) / l_run : 0.f;
+      const float lse2 = l_run > 0.f ? m_ref + fast_log2(l_run) : -INFINITY;
+      const int64_t row = (int64_t)((c.cu ? off : b * c.n) + i_tok) * c.Hq + head;
+      T* orow = (T*)p.o + (c.cu ? (int64_t)(off + i_tok) * p.o_ss : b * p.o_sb + i_tok * p.o_ss) + head * p.o_sh;
+      float* part = p.part_o + (row * p.splits + split) * D;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = db * 32 + i * 8 + hh * 4;
+          const f32x4 x = f32x4{oacc[db][4 * i], oacc[db][4 * i + 1], oacc[db][4 * i + 2], oacc[db][4 * i + 3]} * f;
+          if (p.splits > 1) *reinterpret_cast<f32x4*>(part + d) = x;
+          else *reinterpret_cast<vec4<T>*>(orow + d) = vec4<T>{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+        }
+      if (hh == 0) {
+        if (p.splits > 1) p.part_m[row * p.splits + split] = lse2;
+        else if (p.lse) p.lse[row] = lse2 * kLn2;
+      }
+    }
+  }
+}
+
 // Attention of one token i and query head h of sequence b by one wave, row after row: for tokens
 // past the stated longest sequence, which the grid of the split kernel has no columns for.
 template <class T, bool FP8, int D>
@@ -858,10 +1125,12 @@ paged_combine_kernel(PagedAttnParams p) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int b = 0, i = 0, ns = 0;
   const bool in = token_place(c, t, b, i);
-  const bool alone = in && i >= c.n;   // past the stated longest sequence
+  const bool alone = in && !p.splits && i >= c.n;   // past the stated longest sequence
   const int G = c.Hq / c.Hkv;
-  int64_t base = 0;
-  if (in && !alone) {   // this sequence's pieces
+  int64_t base = 0, step = (int64_t)c.Hkv * p.cols;
+  if (in && p.splits) {          // of the tile kernel, which writes every one
+    ns = p.splits, step = 1, base = ((int64_t)t * c.Hq + h) * p.splits;
+  } else if (in && !alone) {   // this sequence's pieces
     int64_t units = 0, first = 0;
     int mine = 0;
     for (int at = 0; at < c.B; at += 64) {
@@ -881,7 +1150,7 @@ paged_combine_kernel(PagedAttnParams p) {
       base = ((int64_t)(g0 + b) * c.Hkv + h / G) * p.cols + i * G + h % G;
     }
   }
-  const int64_t row = (int64_t)t * c.Hq + h, step = (int64_t)c.Hkv * p.cols;
+  const int64_t row = (int64_t)t * c.Hq + h;
   float acc[DJ];
 #pragma unroll
   for (int j = 0; j < DJ; ++j) acc[j] = 0.f;
@@ -935,6 +1204,9 @@ paged_combine_kernel(PagedAttnParams p) {
   if (p.lse && threadIdx.x == 0) p.lse[row] = sum > 0.f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
 }
 
+#ifndef FAL_PAGED_TILE_FROM
+#define FAL_PAGED_TILE_FROM 32
+#endif
 #ifndef FAL_PAGED_WH
 #define FAL_PAGED_WH 4
 #endif
@@ -950,6 +1222,18 @@ paged_combine_kernel(PagedAttnParams p) {
 PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
                      int row_bytes, int ncu) {
   PagedPlan r{};
+  r.max_cols = FAL_PAGED_TILE_FROM;
+  const int64_t wide = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
+  if (wide > r.max_cols) {
+    const int64_t tiles = (wide + kTileCols - 1) / kTileCols;
+    r.tile_cols = (int)tiles;
+    const int64_t blocks = B * Hkv * tiles, slots = (int64_t)ncu * (d > 128 ? 1 : 2);
+    const int64_t longest = (capacity + 4 * kTileRows - 1) / (4 * kTileRows);   // (four tiles at least)
+    int64_t n = slots / (blocks > 0 ? blocks : 1);
+    n = n > 16 ? 16 : n > longest ? longest : n;
+    r.splits = (int)(n < 1 ? 1 : n);
+    return r;
+  }
   const int waves = paged_waves(d, fp8);
   const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
   r.nc = cols <= 16 || d > 128 ? 1 : 2;   // (head dim 256: two tiles would not fit the registers)
@@ -968,6 +1252,14 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t
 
 template <class T, bool FP8, int D>
 static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
+  if (p.splits) {
+    hipLaunchKernelGGL((paged_tile_kernel<T, FP8, D>), dim3((unsigned)(p.tile_blocks + (p.splits > 1 ? 0 : p.rest_blocks))),
+                       dim3(256), 0, st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(256), 0, st, p);
+    return hipGetLastError();
+  }
   const dim3 grid((unsigned)(p.parts * (p.c.Hkv / p.wave_heads) * p.col_tiles)), block(paged_waves(D, FP8) * 64);
   if (D > 128 || p.nc == 1) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((paged_split_kernel<T, FP8, (D > 128 ? 128 : D), 2>), grid, block, 0, st, p);
