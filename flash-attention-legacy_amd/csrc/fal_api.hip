@@ -818,9 +818,10 @@ int check_cache(const char* name, const fal_paged_cache& c, const void* p, const
   const int64_t bytes = c.fp8 ? 1 : 2;
   if (!p && c.num_pages > 0) return fail(FAL_ERR_INVALID, "%s: null pointer", name);
   if (!aligned16(p)) return fail(FAL_ERR_INVALID, "%s: base pointer must be 16-byte aligned", name);
+  // (kernels multiply page numbers by 32-bit strides in units of 16 bytes)
   for (int i = 0; i < 3; ++i)
-    if (st[i] < 0 || st[i] * bytes % 16 != 0)
-      return fail(FAL_ERR_INVALID, "%s: stride[%d]=%lld must be a non-negative multiple of 16 bytes", name, i,
+    if (st[i] < 0 || st[i] > (int64_t(1) << 33) || st[i] * bytes % 16 != 0)
+      return fail(FAL_ERR_INVALID, "%s: stride[%d]=%lld must be a non-negative multiple of 16 bytes up to 2^33", name, i,
                   (long long)st[i]);
   // kernels address the rows of a page with 32-bit byte offsets
   if (st[2] >= (int64_t(1) << 22))
@@ -840,7 +841,6 @@ int check_cache(const char* name, const fal_paged_cache& c, const void* p, const
     if (a.stride < span)
       return fail(FAL_ERR_INVALID, "%s: rows overlap (stride %lld over %lld elements)", name, (long long)a.stride,
                   (long long)span);
-    if (a.stride > (int64_t(1) << 61) / a.size) return fail(FAL_ERR_INVALID, "%s: stride too large", name);
     span += a.stride * (a.size - 1);
   }
   return FAL_OK;
@@ -850,7 +850,8 @@ int check_scale(const char* name, const fal_paged_cache& c, const float* p, cons
   if (!c.fp8) return p ? fail(FAL_ERR_INVALID, "%s: a 16-bit cache has no scales", name) : FAL_OK;
   if (!p && c.num_pages > 0) return fail(FAL_ERR_INVALID, "%s: null pointer", name);
   if (reinterpret_cast<uintptr_t>(p) & 3) return fail(FAL_ERR_INVALID, "%s: base pointer must be 4-byte aligned", name);
-  if (st[0] < 0 || st[1] < 0) return fail(FAL_ERR_INVALID, "%s: negative stride", name);
+  if (st[0] < 0 || st[1] < 0 || st[0] > 0x7fffffff || st[1] > 0x7fffffff)
+    return fail(FAL_ERR_INVALID, "%s: strides must be non-negative and below 2^31", name);
   if (!written) return FAL_OK;
   const bool by_page = st[0] >= st[1];   // which axis is the outer one
   const int64_t inner = by_page ? st[1] : st[0], outer = by_page ? st[0] : st[1];

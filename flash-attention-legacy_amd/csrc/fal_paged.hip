@@ -850,6 +850,12 @@ paged_tile_kernel(PagedAttnParams p) {
   int off, len;
   token_range(c, b, off, len);
   const int L = cache_rows(c, b), ncols = len * G;
+  const char* const kbase = (const char*)c.k + hkv * c.k_sh * CB;
+  const char* const vbase = (const char*)c.v + hkv * c.v_sh * CB;
+  const float* const kscale = FP8 ? c.k_scale + hkv * c.ks_sh : nullptr;
+  const float* const vscale = FP8 ? c.v_scale + hkv * c.vs_sh : nullptr;
+  const uint32_t k_page = (uint32_t)(c.k_sp * CB >> 4), v_page = (uint32_t)(c.v_sp * CB >> 4);   // 16-byte units
+  const int step_pages = kTileRows / c.page_size, step_rows = kTileRows - step_pages * c.page_size;
   // column tiles, those that see the most rows first; past the stated longest sequence each
   // workgroup takes further ones
   for (int ct = p.tile_cols - 1 - rest / p.splits; ct * kTileCols < ncols; ct += p.tile_cols) {
@@ -884,33 +890,38 @@ paged_tile_kernel(PagedAttnParams p) {
       kv[i] = r < 16 ? r * k_ss + u * 16 : 0x7ffffff0;
       vv[i] = r < 16 ? r * v_ss + u * 16 : 0x7ffffff0;
     }
-    auto page_of = [&](int tile) {   // page number of this wave's slice, -1: none
-      const int r = tile * kTileRows + w * 16;
-      if (tile >= t1 || r >= k_hi) return -1;
-      const int pid = c.table[b * c.table_sb + r / c.page_size];
-      return pid >= 0 && pid < c.num_pages ? pid : -1;
+    // the wave's slice of the tile whose page number is asked for next: its first row, and that
+    // row's page and place in it
+    int row = t0 * kTileRows + w * 16, page = row / c.page_size, slot = row - page * c.page_size;
+    struct Slice { int pid, slot, rows; };
+    auto next_slice = [&]() {
+      Slice x{-1, slot, 0};
+      if (row < min(k_hi, t1 * kTileRows)) {
+        const int pid = c.table[b * c.table_sb + page];
+        if (pid >= 0 && pid < c.num_pages) x.pid = pid, x.rows = min(16, k_hi - row);
+      }
+      row += kTileRows, page += step_pages, slot += step_rows;
+      if (slot >= c.page_size) slot -= c.page_size, ++page;
+      return x;
     };
     u32x4 kreg[LOADS], vreg[LOADS];
     float ksc = 1.f, vsc = 1.f;
-    auto fetch = [&](int tile, int pid) {
-      const int r = tile * kTileRows + w * 16, slot = r % c.page_size;
-      const int n = pid >= 0 ? min(16, k_hi - r) : 0;
-      const int64_t at = pid >= 0 ? pid : 0;
-      const auto krs = make_rsrc((const char*)c.k + (at * c.k_sp + hkv * c.k_sh + slot * c.k_ss) * CB,
-                                 n > 0 ? (uint32_t)((n - 1) * k_ss + RB) : 0);
-      const auto vrs = make_rsrc((const char*)c.v + (at * c.v_sp + hkv * c.v_sh + slot * c.v_ss) * CB,
-                                 n > 0 ? (uint32_t)((n - 1) * v_ss + RB) : 0);
+    auto fetch = [&](Slice x) {
+      const uint32_t pid = x.pid >= 0 ? x.pid : 0;
+      const auto krs = make_rsrc(kbase + ((uint64_t)pid * k_page << 4) + (uint32_t)(x.slot * k_ss),
+                                 x.rows > 0 ? (uint32_t)((x.rows - 1) * k_ss + RB) : 0);
+      const auto vrs = make_rsrc(vbase + ((uint64_t)pid * v_page << 4) + (uint32_t)(x.slot * v_ss),
+                                 x.rows > 0 ? (uint32_t)((x.rows - 1) * v_ss + RB) : 0);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         kreg[i] = __builtin_amdgcn_raw_buffer_load_b128(krs, kv[i], 0, 0);
         vreg[i] = __builtin_amdgcn_raw_buffer_load_b128(vrs, vv[i], 0, 0);
       }
-      if (FP8 && n > 0) {
-        ksc = c.k_scale[pid * c.ks_sp + hkv * c.ks_sh];
-        vsc = c.v_scale[pid * c.vs_sp + hkv * c.vs_sh];
+      vsc = x.rows > 0 ? 1.f : -1.f;
+      if (FP8 && x.rows > 0) {
+        ksc = kscale[(uint64_t)pid * (uint32_t)c.ks_sp];
+        vsc = vscale[(uint64_t)pid * (uint32_t)c.vs_sp];
       }
-      if (n <= 0) vsc = -1.f;
-      else if (!FP8) vsc = 1.f;
     };
     auto stage = [&](int buf) {
 #pragma unroll
@@ -932,24 +943,47 @@ paged_tile_kernel(PagedAttnParams p) {
     };
 
     if (t0 < t1) {
-      int pid = page_of(t0 + 1);
-      fetch(t0, page_of(t0));
+      const Slice s0 = next_slice(), s1 = next_slice();
+      Slice coming = next_slice();
+      fetch(s0);
       stage(0);
-      fetch(t0 + 1, pid);
-      pid = page_of(t0 + 2);
+      fetch(s1);
       __syncthreads();
-      for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
+      auto step = [&](auto bufc, int t) {
+        constexpr int buf = decltype(bufc)::value;
         if (active) {
           // S^T: element i of block mb is row mb * 32 + (i / 4) * 8 + hh * 4 + i % 4, column l32
-          f32x16 s[2];
+          f32x16 s[2] = {zero_f16(), zero_f16()};
+          constexpr int KB = 2;   // k-steps whose operands are read together, one group ahead
+          V8 ka[2][2][KB];
+          auto read_k = [&](int g) {
 #pragma unroll
-          for (int mb = 0; mb < 2; ++mb) {
-            s[mb] = zero_f16();
+            for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-              s[mb] = mfma32(ld8(&ksm[buf][Tile::offset(mb * 32 + l32, ks * 2 + hh)]), qreg[ks], s[mb]);
+              for (int i = 0; i < KB; ++i)
+                ka[g & 1][mb][i] = ld8(&ksm[buf][Tile::offset(mb * 32 + l32, (g * KB + i) * 2 + hh)]);
+          };
+          read_k(0);
+#pragma unroll
+          for (int g = 0; g < KS / KB; ++g) {
+            if (g + 1 < KS / KB) read_k(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < KB; ++i)
+#pragma unroll
+              for (int mb = 0; mb < 2; ++mb) s[mb] = mfma32(ka[g & 1][mb][i], qreg[g * KB + i], s[mb]);
           }
+          // V operands of the first slice, read while the softmax runs
+          V8 va[2][DB];
+          const int tr = hh * 4 + ((lane & 15) >> 2), tc = ((lane & 16) >> 3) + ((lane & 3) >> 1);
+          auto read_v = [&](int x) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+              va[x & 1][db] = join8(lds_tr(&vsm[buf][Tile::offset(x * 16 + tr, db * 4 + tc) + (lane & 1) * 4]),
+                                    lds_tr(&vsm[buf][Tile::offset(x * 16 + 8 + tr, db * 4 + tc) + (lane & 1) * 4]));
+          };
+          read_v(0);
+          __builtin_amdgcn_sched_barrier(0);
           // slice x: elements 8 (x % 2) .. + 8 of block x / 2
           float kfac[4], vlog[4], vinv[4], back = 1.f;
           bool whole = (t + 1) * kTileRows <= lim_first;
@@ -993,8 +1027,9 @@ paged_tile_kernel(PagedAttnParams p) {
           for (int x = 0; x < 4; ++x) {
             const f32x16& y = s[x / 2];
             const int o = (x & 1) * 8;
-            const float a = fmaxf(fmaxf(fmaxf(y[o], y[o + 1]), fmaxf(y[o + 2], y[o + 3])),
-                                  fmaxf(fmaxf(y[o + 4], y[o + 5]), fmaxf(y[o + 6], y[o + 7])));
+            float a = y[o];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) a = __builtin_elementwise_maximum(a, y[o + i]);
             mx = fmaxf(mx, a * kfac[x]);
           }
           mx = pair_max(mx);
@@ -1022,22 +1057,25 @@ paged_tile_kernel(PagedAttnParams p) {
             l_run = FP8 ? fmaf(l, vinv[x], l_run) : l_run + l;
           }
           // O^T += V^T P^T
-          const int tr = hh * 4 + ((lane & 15) >> 2), tc = ((lane & 16) >> 3) + ((lane & 3) >> 1);
 #pragma unroll
-          for (int db = 0; db < DB; ++db)
+          for (int x = 0; x < 4; ++x) {
+            if (x < 3) read_v(x + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const V8 a = join8(lds_tr(&vsm[buf][Tile::offset(x * 16 + tr, db * 4 + tc) + (lane & 1) * 4]),
-                                 lds_tr(&vsm[buf][Tile::offset(x * 16 + 8 + tr, db * 4 + tc) + (lane & 1) * 4]));
-              oacc[db] = mfma32(a, pb[x], oacc[db]);
-            }
+            for (int db = 0; db < DB; ++db) oacc[db] = mfma32(va[x & 1][db], pb[x], oacc[db]);
+          }
         }
         if (t + 1 < t1) {
           stage(buf ^ 1);
-          fetch(t + 2, pid);
-          pid = page_of(t + 3);
+          fetch(coming);
+          coming = next_slice();
         }
         __syncthreads();
+      };
+      // two tiles per trip so that the buffer is a compile-time constant
+      for (int t = t0; t < t1; t += 2) {
+        step(std::integral_constant<int, 0>{}, t);
+        if (t + 1 < t1) step(std::integral_constant<int, 1>{}, t + 1);
       }
     }
 
@@ -1125,12 +1163,10 @@ paged_combine_kernel(PagedAttnParams p) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int b = 0, i = 0, ns = 0;
   const bool in = token_place(c, t, b, i);
-  const bool alone = in && !p.splits && i >= c.n;   // past the stated longest sequence
+  const bool alone = in && i >= c.n;   // past the stated longest sequence
   const int G = c.Hq / c.Hkv;
   int64_t base = 0, step = (int64_t)c.Hkv * p.cols;
-  if (in && p.splits) {          // of the tile kernel, which writes every one
-    ns = p.splits, step = 1, base = ((int64_t)t * c.Hq + h) * p.splits;
-  } else if (in && !alone) {   // this sequence's pieces
+  if (in && !alone) {   // this sequence's pieces
     int64_t units = 0, first = 0;
     int mine = 0;
     for (int at = 0; at < c.B; at += 64) {
@@ -1204,6 +1240,37 @@ paged_combine_kernel(PagedAttnParams p) {
   if (p.lse && threadIdx.x == 0) p.lse[row] = sum > 0.f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
 }
 
+// Merge the tile kernel's splits, four elements of one (token, query head) per thread.
+template <class T, int D>
+__global__ void __launch_bounds__(256)
+paged_merge_kernel(PagedAttnParams p) {
+  const PagedCache& c = p.c;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / (D / 4);
+  const int d = (int)(i % (D / 4)) * 4;
+  if (row >= (int64_t)c.total * c.Hq) return;
+  const int t = (int)(row / c.Hq), h = (int)(row % c.Hq);
+  int b, n;
+  const bool in = token_place(c, t, b, n);
+  const float* pm = p.part_m + row * p.splits;
+  const f32x4* po = reinterpret_cast<const f32x4*>(p.part_o + row * p.splits * D + d);
+  float M = -INFINITY, sum = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (in) {
+    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, pm[s]);
+    if (M > -INFINITY)
+      for (int s = 0; s < p.splits; ++s) {
+        const float w = fast_exp2(pm[s] - M);
+        sum += w;
+        o += po[s * (D / 4)] * w;
+      }
+  }
+  o *= sum > 0.f ? 1.f / sum : 0.f;
+  T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + n * p.o_ss) + h * p.o_sh;
+  *reinterpret_cast<vec4<T>*>(orow + d) = vec4<T>{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
+  if (p.lse && d == 0) p.lse[row] = sum > 0.f ? (M + fast_log2(sum)) * kLn2 : -INFINITY;
+}
+
 #ifndef FAL_PAGED_TILE_FROM
 #define FAL_PAGED_TILE_FROM 32
 #endif
@@ -1257,7 +1324,8 @@ static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
                        dim3(256), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(256), 0, st, p);
+    const int64_t threads = (int64_t)p.c.total * p.c.Hq * (D / 4);
+    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, p);
     return hipGetLastError();
   }
   const dim3 grid((unsigned)(p.parts * (p.c.Hkv / p.wave_heads) * p.col_tiles)), block(paged_waves(D, FP8) * 64);

@@ -68,11 +68,13 @@ BAD_CACHES = [
     (dict(v=P + 8), FAL_ERR_INVALID, "v_cache: base pointer must be 16-byte aligned"),
     (dict(k_strides=(16384, 128, 264)), FAL_ERR_INVALID, "k_cache: stride[2]=264 must be a non-negative multiple of 16 bytes"),
     (dict(v_strides=(-16384, 128, 256)), FAL_ERR_INVALID, "v_cache: stride[0]"),
+    (dict(k_strides=(2 ** 33 + 16, 128, 256)), FAL_ERR_INVALID, "k_cache: stride[0]"),
+    (dict(k_scale_strides=(2 ** 31, 1)), FAL_ERR_INVALID, "k_scale: strides must be"),
     (dict(v_strides=(2 ** 30, 128, 2 ** 22)), FAL_ERR_UNSUPPORTED, "v_cache: row stride"),
     (dict(v_strides=(16384, 128, 112)), FAL_ERR_UNSUPPORTED, "shorter than a row"),
     (dict(k_scale=None), FAL_ERR_INVALID, "k_scale: null pointer"),
     (dict(v_scale=P + 2), FAL_ERR_INVALID, "v_scale: base pointer must be 4-byte aligned"),
-    (dict(v_scale_strides=(-2, 1)), FAL_ERR_INVALID, "v_scale: negative stride"),
+    (dict(v_scale_strides=(-2, 1)), FAL_ERR_INVALID, "v_scale: strides must be non-negative"),
     (dict(fp8=0, k_strides=(32768, 128, 256), v_strides=(32768, 128, 256)), FAL_ERR_INVALID, "a 16-bit cache has no scales"),
 ]
 
