@@ -802,9 +802,9 @@ paged_split_kernel(PagedAttnParams p) {
 // Attention, many columns: tiles of keys shared by a workgroup
 // ---------------------------------------------------------------------------
 // One workgroup takes 128 columns (see above) of one sequence and KV head, 32 to a wave, and
-// walks tiles of 64 rows; with few workgroups, `splits` of them share a column tile's rows.
-// * Wave w brings the tile's slice w (16 rows of one page) from the cache: its page and scales
-//   are scalars, its lanes' places in the page constants, and e4m3 codes become 16-bit values
+// walks tiles of 64 or 32 rows; with few workgroups, `splits` of them share a column tile's rows.
+// * Each wave brings a slice of the tile (16 rows of one page, or half of one) from the cache: its
+//   page and scales are scalars, its lanes' places in the page constants, and e4m3 codes become 16-bit values
 //   once, on the way to LDS, not once per wave that reads them.  Loads of a tile run a whole
 //   tile ahead, its page number two.
 // * S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMA; the S^T accumulators are P^T's operand in
@@ -813,19 +813,22 @@ paged_split_kernel(PagedAttnParams p) {
 //   P reaches 2^8 at most, and the accumulators are rarely rescaled.
 // * Scales as in the split kernel: the value factor enters the exponent, and each slice's sum is
 //   divided by it again for l.
-constexpr int kTileRows = 64, kTileCols = 128;
+constexpr int kTileCols = 128;
+constexpr int tile_rows(int d) { return d > 128 ? 32 : 64; }   // (head dim 256: registers)
 
 template <class T, bool FP8, int D>
 __global__ void __launch_bounds__(256, D > 128 ? 1 : 2)
 paged_tile_kernel(PagedAttnParams p) {
   constexpr int DB = D / 32, KS = D / 16;
   constexpr int RB = FP8 ? D : 2 * D, CPR = RB / 16;         // bytes of a cache row, its 16-byte pieces
-  constexpr int LOADS = (16 * CPR + 63) / 64;                // pieces per lane of a slice
+  constexpr int TR = tile_rows(D), NS = TR / 16;             // rows and slices of a tile
+  constexpr int RW = TR / 4;                                 // rows that a wave brings
+  constexpr int LOADS = (RW * CPR + 63) / 64;                // pieces per lane of those
   constexpr int CB = FP8 ? 1 : 2;
   using V8 = vec8<T>;
   using Tile = SwizzledTile<D>;
-  __shared__ __attribute__((aligned(1024))) T ksm[2][kTileRows * D], vsm[2][kTileRows * D];
-  __shared__ float ssm[2][4][2];                             // per slice: key and value scale (-1: no page)
+  __shared__ __attribute__((aligned(1024))) T ksm[2][TR * D], vsm[2][TR * D];
+  __shared__ float ssm[2][NS][2];                             // per slice: key and value scale (-1: no page)
 
   const PagedCache& c = p.c;
   const int G = c.Hq / c.Hkv;
@@ -855,13 +858,13 @@ paged_tile_kernel(PagedAttnParams p) {
   const float* const kscale = FP8 ? c.k_scale + hkv * c.ks_sh : nullptr;
   const float* const vscale = FP8 ? c.v_scale + hkv * c.vs_sh : nullptr;
   const uint32_t k_page = (uint32_t)(c.k_sp * CB >> 4), v_page = (uint32_t)(c.v_sp * CB >> 4);   // 16-byte units
-  const int step_pages = kTileRows / c.page_size, step_rows = kTileRows - step_pages * c.page_size;
+  const int step_pages = TR / c.page_size, step_rows = TR - step_pages * c.page_size;
   // column tiles, those that see the most rows first; past the stated longest sequence each
   // workgroup takes further ones
   for (int ct = p.tile_cols - 1 - rest / p.splits; ct * kTileCols < ncols; ct += p.tile_cols) {
     const int col_last = min(ncols, (ct + 1) * kTileCols) - 1;
     const int k_hi = max(p.causal ? L - len + col_last / G + 1 : L, 0);
-    const int tiles = cdiv(k_hi, kTileRows);
+    const int tiles = cdiv(k_hi, TR);
     const int t0 = (int)((int64_t)tiles * split / p.splits), t1 = (int)((int64_t)tiles * (split + 1) / p.splits);
 
     // this wave's columns
@@ -887,20 +890,20 @@ paged_tile_kernel(PagedAttnParams p) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int e = i * 64 + lane, r = e / CPR, u = e % CPR;
-      kv[i] = r < 16 ? r * k_ss + u * 16 : 0x7ffffff0;
-      vv[i] = r < 16 ? r * v_ss + u * 16 : 0x7ffffff0;
+      kv[i] = r < RW ? r * k_ss + u * 16 : 0x7ffffff0;
+      vv[i] = r < RW ? r * v_ss + u * 16 : 0x7ffffff0;
     }
     // the wave's slice of the tile whose page number is asked for next: its first row, and that
     // row's page and place in it
-    int row = t0 * kTileRows + w * 16, page = row / c.page_size, slot = row - page * c.page_size;
+    int row = t0 * TR + w * RW, page = row / c.page_size, slot = row - page * c.page_size;
     struct Slice { int pid, slot, rows; };
     auto next_slice = [&]() {
       Slice x{-1, slot, 0};
-      if (row < min(k_hi, t1 * kTileRows)) {
+      if (row < min(k_hi, t1 * TR)) {
         const int pid = c.table[b * c.table_sb + page];
-        if (pid >= 0 && pid < c.num_pages) x.pid = pid, x.rows = min(16, k_hi - row);
+        if (pid >= 0 && pid < c.num_pages) x.pid = pid, x.rows = min(RW, k_hi - row);
       }
-      row += kTileRows, page += step_pages, slot += step_rows;
+      row += TR, page += step_pages, slot += step_rows;
       if (slot >= c.page_size) slot -= c.page_size, ++page;
       return x;
     };
@@ -926,8 +929,8 @@ paged_tile_kernel(PagedAttnParams p) {
     auto stage = [&](int buf) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int e = i * 64 + lane, r = e / CPR, u = e % CPR, row = w * 16 + r;
-        if (16 * CPR % 64 != 0 && r >= 16) continue;
+        const int e = i * 64 + lane, r = e / CPR, u = e % CPR, row = w * RW + r;
+        if (RW * CPR % 64 != 0 && r >= RW) continue;
         if constexpr (FP8) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
@@ -939,7 +942,7 @@ paged_tile_kernel(PagedAttnParams p) {
           st_u4(&vsm[buf][Tile::offset(row, u)], vreg[i]);
         }
       }
-      if (lane == 0) ssm[buf][w][0] = ksc, ssm[buf][w][1] = vsc;
+      if (lane == 0 && w * RW % 16 == 0) ssm[buf][w * RW / 16][0] = ksc, ssm[buf][w * RW / 16][1] = vsc;
     };
 
     if (t0 < t1) {
@@ -953,12 +956,15 @@ paged_tile_kernel(PagedAttnParams p) {
         constexpr int buf = decltype(bufc)::value;
         if (active) {
           // S^T: element i of block mb is row mb * 32 + (i / 4) * 8 + hh * 4 + i % 4, column l32
-          f32x16 s[2] = {zero_f16(), zero_f16()};
+          constexpr int MB = TR / 32;
+          f32x16 s[MB];
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) s[mb] = zero_f16();
           constexpr int KB = 2;   // k-steps whose operands are read together, one group ahead
-          V8 ka[2][2][KB];
+          V8 ka[2][MB][KB];
           auto read_k = [&](int g) {
 #pragma unroll
-            for (int mb = 0; mb < 2; ++mb)
+            for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
               for (int i = 0; i < KB; ++i)
                 ka[g & 1][mb][i] = ld8(&ksm[buf][Tile::offset(mb * 32 + l32, (g * KB + i) * 2 + hh)]);
@@ -971,26 +977,30 @@ paged_tile_kernel(PagedAttnParams p) {
 #pragma unroll
             for (int i = 0; i < KB; ++i)
 #pragma unroll
-              for (int mb = 0; mb < 2; ++mb) s[mb] = mfma32(ka[g & 1][mb][i], qreg[g * KB + i], s[mb]);
+              for (int mb = 0; mb < MB; ++mb) s[mb] = mfma32(ka[g & 1][mb][i], qreg[g * KB + i], s[mb]);
           }
           // V operands of the first slice, read while the softmax runs
-          V8 va[2][DB];
+          constexpr int VG = DB < 4 ? DB : 4, VH = DB / VG;   // head-dim blocks read together, groups of them
+          V8 va[2][VG];
           const int tr = hh * 4 + ((lane & 15) >> 2), tc = ((lane & 16) >> 3) + ((lane & 3) >> 1);
-          auto read_v = [&](int x) {
+          auto read_v = [&](int g) {
+            const int x = g / VH;
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-              va[x & 1][db] = join8(lds_tr(&vsm[buf][Tile::offset(x * 16 + tr, db * 4 + tc) + (lane & 1) * 4]),
-                                    lds_tr(&vsm[buf][Tile::offset(x * 16 + 8 + tr, db * 4 + tc) + (lane & 1) * 4]));
+            for (int i = 0; i < VG; ++i) {
+              const int ch = (g % VH * VG + i) * 4 + tc;
+              va[g & 1][i] = join8(lds_tr(&vsm[buf][Tile::offset(x * 16 + tr, ch) + (lane & 1) * 4]),
+                                   lds_tr(&vsm[buf][Tile::offset(x * 16 + 8 + tr, ch) + (lane & 1) * 4]));
+            }
           };
           read_v(0);
           __builtin_amdgcn_sched_barrier(0);
           // slice x: elements 8 (x % 2) .. + 8 of block x / 2
-          float kfac[4], vlog[4], vinv[4], back = 1.f;
-          bool whole = (t + 1) * kTileRows <= lim_first;
+          float kfac[NS], vlog[NS], vinv[NS], back = 1.f;
+          bool whole = (t + 1) * TR <= lim_first;
           if constexpr (FP8) {
-            float v[4], now = ref;
+            float v[NS], now = ref;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < NS; ++x) {
               kfac[x] = fmaxf(p.scale_log2 * ssm[buf][x][0], 0x1p-126f);
               v[x] = ssm[buf][x][1];
               whole = whole && __builtin_amdgcn_readfirstlane(__float_as_int(v[x])) >= 0;
@@ -1000,31 +1010,31 @@ paged_tile_kernel(PagedAttnParams p) {
             back = ref * inv;
             ref = now;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {   // (a value scale 2^60 below the largest counts as that)
+            for (int x = 0; x < NS; ++x) {   // (a value scale 2^60 below the largest counts as that)
               const float f = fmaxf(v[x] * inv, 0x1p-60f);
               vlog[x] = fast_log2(f), vinv[x] = __builtin_amdgcn_rcpf(f);
             }
           } else {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < NS; ++x) {
               kfac[x] = p.scale_log2, vlog[x] = 0.f, vinv[x] = 1.f;
               whole = whole && __builtin_amdgcn_readfirstlane(__float_as_int(ssm[buf][x][1])) >= 0;
             }
           }
           if (!whole) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < NS; ++x) {
               const bool none = ssm[buf][x][1] < 0.f;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const int r = t * kTileRows + x * 16 + (i / 4) * 8 + hh * 4 + i % 4;
+                const int r = t * TR + x * 16 + (i / 4) * 8 + hh * 4 + i % 4;
                 if (none || r >= lim) s[x / 2][(x & 1) * 8 + i] = -INFINITY;
               }
             }
           }
           float mx = -INFINITY;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < NS; ++x) {
             const f32x16& y = s[x / 2];
             const int o = (x & 1) * 8;
             float a = y[o];
@@ -1043,9 +1053,9 @@ paged_tile_kernel(PagedAttnParams p) {
             for (int i = 0; i < DB; ++i) oacc[i] *= f;
           }
           const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-          V8 pb[4];
+          V8 pb[NS];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < NS; ++x) {
             const float sub = FP8 ? vlog[x] - m_use : -m_use;
             float l = 0.f;
 #pragma unroll
@@ -1058,11 +1068,12 @@ paged_tile_kernel(PagedAttnParams p) {
           }
           // O^T += V^T P^T
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (x < 3) read_v(x + 1);
+          for (int g = 0; g < NS * VH; ++g) {
+            if (g + 1 < NS * VH) read_v(g + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int db = 0; db < DB; ++db) oacc[db] = mfma32(va[x & 1][db], pb[x], oacc[db]);
+            for (int i = 0; i < VG; ++i)
+              oacc[g % VH * VG + i] = mfma32(va[g & 1][i], pb[g / VH], oacc[g % VH * VG + i]);
           }
         }
         if (t + 1 < t1) {
@@ -1295,7 +1306,7 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t
     const int64_t tiles = (wide + kTileCols - 1) / kTileCols;
     r.tile_cols = (int)tiles;
     const int64_t blocks = B * Hkv * tiles, slots = (int64_t)ncu * (d > 128 ? 1 : 2);
-    const int64_t longest = (capacity + 4 * kTileRows - 1) / (4 * kTileRows);   // (four tiles at least)
+    const int64_t longest = (capacity + 4 * tile_rows(d) - 1) / (4 * tile_rows(d));   // (four tiles at least)
     int64_t n = slots / (blocks > 0 ? blocks : 1);
     n = n > 16 ? 16 : n > longest ? longest : n;
     r.splits = (int)(n < 1 ? 1 : n);
