@@ -171,7 +171,8 @@ struct PagedAppendParams {
   int64_t k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, q_sb, q_sh, q_ss, qo_sb, qo_sh, qo_ss;
   int64_t cos_ss, sin_ss;
   int rotary, interleaved;
-  int pages_per_seq;  // store blocks per sequence (each walks the touched pages this far apart)
+  int pages_per_seq;  // 8-bit store blocks per sequence (each walks the touched pages this far apart)
+  int row_groups;     // groups of heads of a token that are stored row by row
 };
 
 // Attention over the pages (fal_paged.hip).

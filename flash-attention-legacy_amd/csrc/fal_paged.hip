@@ -46,47 +46,47 @@ __device__ __forceinline__ bool token_place(const PagedCache& c, int t, int& b, 
 // Append
 // ---------------------------------------------------------------------------
 
-// Two chunks of eight elements of a row, rotated where the rotation covers them.  Unit u of a
-// row of D elements: in half-split pairs (x_j, x_{j + r/2}) the chunks u and u + r/16 for
-// u < r/16, and otherwise the chunks 2u and 2u + 1, which hold the interleaved pairs; both use
-// the angles 8u .. 8u + 7.  The products and the sum are rounded one by one (no contraction),
-// so the values do not depend on the compiler's choice.
-template <class T>
-__device__ __forceinline__ void load_unit(const T* row, int u, int rotary, int interleaved, const float* cs,
-                                          const float* sn, int& ca, int& cb, float (&y)[16]) {
-#pragma clang fp contract(off)
-  const bool rot = u * 16 < rotary;
-  const bool halves = rot && !interleaved;
+enum { kNoRotation, kHalves, kInterleaved };
+
+// The chunks (eight elements) of unit u of a row: chunks u and u + r/16 of the half-split pairs
+// (x_j, x_{j + r/2}) for u < r/16, and otherwise 2u and 2u + 1, which hold the interleaved pairs.
+// A unit's pairs use the angles 8u .. 8u + 7 either way.
+template <int MODE>
+__device__ __forceinline__ void unit_chunks(int u, int rotary, int& ca, int& cb) {
+  const bool halves = MODE == kHalves && u * 16 < rotary;
   ca = halves ? u : 2 * u;
   cb = halves ? u + rotary / 16 : 2 * u + 1;
-  const vec8<T> a = ld8(row + ca * 8), b = ld8(row + cb * 8);
-  if (!rot) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = (float)a[j], y[8 + j] = (float)b[j];
-    return;
-  }
+}
+struct Angles {
   f32x4 c[2], s[2];
+};
+template <int MODE>
+__device__ __forceinline__ Angles unit_angles(int u, int rotary, const float* cs, const float* sn) {
+  Angles t;
+  if (MODE == kNoRotation || u * 16 >= rotary) return t;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    c[j] = *reinterpret_cast<const f32x4*>(cs + u * 8 + 4 * j);
-    s[j] = *reinterpret_cast<const f32x4*>(sn + u * 8 + 4 * j);
+    t.c[j] = *reinterpret_cast<const f32x4*>(cs + u * 8 + 4 * j);
+    t.s[j] = *reinterpret_cast<const f32x4*>(sn + u * 8 + 4 * j);
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float cj = c[j / 4][j % 4], sj = s[j / 4][j % 4];
-    // pair j: elements (j, 8 + j) of the two chunks, or (2j, 2j + 1) of the sixteen
-    const float x1 = halves ? (float)a[j] : (float)(j < 4 ? a[2 * j & 7] : b[2 * j & 7]);
-    const float x2 = halves ? (float)b[j] : (float)(j < 4 ? a[(2 * j + 1) & 7] : b[(2 * j + 1) & 7]);
-    const float p1 = x1 * cj, p2 = x2 * sj, p3 = x2 * cj, p4 = x1 * sj;
-    const float y1 = p1 - p2, y2 = p3 + p4;
-    if (halves) y[j] = y1, y[8 + j] = y2;
-    else y[2 * j] = y1, y[2 * j + 1] = y2;
-  }
+  return t;
 }
 
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a < INFINITY ? a : 0.f;   // NaN and infinity: 0
+// The unit's sixteen values, rotated where the rotation covers them.  The products and the sum
+// are rounded one by one (no contraction), so the values do not depend on the compiler's choice.
+template <int MODE, class T, int D>
+__device__ __forceinline__ void rotate_unit(vec8<T> a, vec8<T> b, int u, int rotary, const Angles& t, float (&y)[16]) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = (float)a[j], y[8 + j] = (float)b[j];
+  if (MODE == kNoRotation || (rotary < D && u * 16 >= rotary)) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i1 = MODE == kHalves ? j : 2 * j, i2 = MODE == kHalves ? 8 + j : 2 * j + 1;
+    const float cj = t.c[j / 4][j % 4], sj = t.s[j / 4][j % 4], x1 = y[i1], x2 = y[i2];
+    const float p1 = x1 * cj, p2 = x2 * sj, p3 = x2 * cj, p4 = x1 * sj;
+    y[i1] = p1 - p2, y[i2] = p3 + p4;
+  }
 }
 
 // The smallest 2^e, e >= -126, with amax <= 448 * 2^e (448 = 0.875 * 2^9).
@@ -97,20 +97,17 @@ __device__ __forceinline__ float page_scale(float amax) {
   return ldexpf(1.f, max(e, kMinScaleExp));
 }
 
-// Saturated to +-448 (infinities too; NaN stays NaN)
-__device__ __forceinline__ float e4m3_sat(float x) {
-  return x != x ? x : fminf(fmaxf(x, -kE4m3Max), kE4m3Max);
-}
+// Values of at most 448 in magnitude (or NaN) as codes
 __device__ __forceinline__ uint32_t e4m3_pack4(float a, float b, float c, float d) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_sat(a), e4m3_sat(b), 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_sat(c), e4m3_sat(d), r, true);
+  const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 __device__ __forceinline__ void e4m3_unpack4(uint32_t x, float (&y)[4]) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, true);
   y[0] = lo[0], y[1] = lo[1], y[2] = hi[0], y[3] = hi[1];
 }
 
-// 8 values of a chunk to the cache row
+// 8 values of a chunk to a 16-bit row, or as codes in units of 1 / inv
 template <class T>
 __device__ __forceinline__ void put_chunk(T* row, int chunk, const float* y) {
   vec8<T> r;
@@ -118,169 +115,260 @@ __device__ __forceinline__ void put_chunk(T* row, int chunk, const float* y) {
   for (int j = 0; j < 8; ++j) r[j] = (T)y[j];
   st_u4(row + chunk * 8, __builtin_bit_cast(u32x4, r));
 }
-__device__ __forceinline__ void put_chunk8(uint8_t* row, int chunk, const float* y, float inv) {
+__device__ __forceinline__ void put_codes(uint8_t* row, int chunk, const float* y, float inv) {
   u32x2 r;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
     r[j] = e4m3_pack4(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv);
   *reinterpret_cast<u32x2*>(row + chunk * 8) = r;
 }
+// y * inv, infinities as the largest code (NaN stays)
+__device__ __forceinline__ void scale_saturated(float (&y)[16], float inv) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float x = y[j] * inv;
+    y[j] = x != x ? x : fminf(fmaxf(x, -kE4m3Max), kE4m3Max);
+  }
+}
 
-// Blocks below `store_blocks`: one touched page of one sequence, KV head and side (K or V).
-// Such a block owns the page's rows and scale for its head, so nothing is atomic and the
-// result does not depend on timing.  The others rotate queries, one unit per thread.
-constexpr int kAppendHold = 4;   // units per thread kept in registers between the two passes
+// Rows to rows: units of one token and position in the row for kRowHeads heads, whose angles are
+// read once.  Queries go to q_out; with a 16-bit cache keys and values go to their pages.
+constexpr int kRowHeads = 4;
 
-template <class T, bool FP8, int D>
-__global__ void __launch_bounds__(256)
-paged_append_kernel(PagedAppendParams p, int store_blocks) {
+template <int MODE, class T, int D>
+__device__ __forceinline__ void copy_heads(const T* src, int64_t src_sh, T* dst, int64_t dst_sh, int heads, int u,
+                                           int rotary, const float* cs, const float* sn) {
+  int ca, cb;
+  unit_chunks<MODE>(u, rotary, ca, cb);
+  vec8<T> a[kRowHeads], b[kRowHeads];
+#pragma unroll
+  for (int i = 0; i < kRowHeads; ++i)
+    if (i < heads) a[i] = ld8(src + i * src_sh + ca * 8), b[i] = ld8(src + i * src_sh + cb * 8);
+  const Angles t = unit_angles<MODE>(u, rotary, cs, sn);
+#pragma unroll
+  for (int i = 0; i < kRowHeads; ++i)
+    if (i < heads) {
+      float y[16];
+      rotate_unit<MODE, T, D>(a[i], b[i], u, rotary, t, y);
+      put_chunk(dst + i * dst_sh, ca, y);
+      put_chunk(dst + i * dst_sh, cb, y + 8);
+    }
+}
+
+template <class T, int D>
+__device__ void append_rows(const PagedAppendParams& p, int64_t item) {
+  constexpr int UPR = D / 16;
+  const PagedCache& c = p.c;
+  const int u = (int)(item % UPR);
+  item /= UPR;
+  const int group = (int)(item % p.row_groups);
+  const int64_t t = item / p.row_groups;
+  if (t >= c.total) return;
+  int b, i;
+  const bool in = token_place(c, (int)t, b, i);
+  const int64_t pos = in ? (int64_t)max(c.seqlens[b], 0) + i : c.capacity;
+  const int qg = p.q ? cdiv(c.Hq, kRowHeads) : 0, kg = cdiv(c.Hkv, kRowHeads);
+  if (group < qg) {
+    const int h = group * kRowHeads, n = min(kRowHeads, c.Hq - h);
+    T* out = (T*)p.q_out + (c.cu ? t * p.qo_ss : b * p.qo_sb + i * p.qo_ss) + h * p.qo_sh;
+    if (pos >= c.capacity) {   // outside every sequence, or past the table
+      for (int x = 0; x < n; ++x) {
+        st_u4(out + x * p.qo_sh + u * 16, u32x4{0, 0, 0, 0});
+        st_u4(out + x * p.qo_sh + u * 16 + 8, u32x4{0, 0, 0, 0});
+      }
+      return;
+    }
+    const T* q = (const T*)p.q + (c.cu ? t * p.q_ss : b * p.q_sb + i * p.q_ss) + h * p.q_sh;
+    const float *cs = p.cos + pos * p.cos_ss, *sn = p.sin + pos * p.sin_ss;
+    if (!p.rotary) copy_heads<kNoRotation, T, D>(q, p.q_sh, out, p.qo_sh, n, u, 0, cs, sn);
+    else if (p.interleaved) copy_heads<kInterleaved, T, D>(q, p.q_sh, out, p.qo_sh, n, u, p.rotary, cs, sn);
+    else copy_heads<kHalves, T, D>(q, p.q_sh, out, p.qo_sh, n, u, p.rotary, cs, sn);
+    return;
+  }
+  if (pos >= c.capacity) return;
+  const int page = (int)(pos / c.page_size), slot = (int)(pos - (int64_t)page * c.page_size);
+  const int pid = c.table[b * c.table_sb + page];
+  if (pid < 0 || pid >= c.num_pages) return;
+  const bool is_v = group - qg >= kg;
+  const int h = (is_v ? group - qg - kg : group - qg) * kRowHeads, n = min(kRowHeads, c.Hkv - h);
+  if (is_v) {
+    const T* v = (const T*)p.v + (c.cu ? t * p.v_ss : b * p.v_sb + i * p.v_ss) + h * p.v_sh;
+    T* to = (T*)c.v + pid * c.v_sp + h * c.v_sh + slot * c.v_ss;
+    copy_heads<kNoRotation, T, D>(v, p.v_sh, to, c.v_sh, n, u, 0, nullptr, nullptr);
+    return;
+  }
+  const T* k = (const T*)p.k + (c.cu ? t * p.k_ss : b * p.k_sb + i * p.k_ss) + h * p.k_sh;
+  T* to = (T*)c.k + pid * c.k_sp + h * c.k_sh + slot * c.k_ss;
+  const float *cs = p.cos + pos * p.cos_ss, *sn = p.sin + pos * p.sin_ss;
+  if (!p.rotary) copy_heads<kNoRotation, T, D>(k, p.k_sh, to, c.k_sh, n, u, 0, cs, sn);
+  else if (p.interleaved) copy_heads<kInterleaved, T, D>(k, p.k_sh, to, c.k_sh, n, u, p.rotary, cs, sn);
+  else copy_heads<kHalves, T, D>(k, p.k_sh, to, c.k_sh, n, u, p.rotary, cs, sn);
+}
+
+// Rows to codes: one touched page of one sequence and KV head, K or V, per workgroup.  It owns
+// the page's rows and scale for its head, so nothing is atomic and the result does not depend on
+// timing.  Two passes, for the largest magnitude and for the codes; each thread keeps its first
+// units in registers between them and reads the others again (from L2).
+constexpr int kAppendHold = 2, kAppendThreads = 512;
+
+template <int MODE, class T, int D>
+__device__ void append_codes(const PagedAppendParams& p, int b, int h, int first_page, const T* src, int64_t src_ss,
+                             uint8_t* cache, int64_t dst_sp, int64_t dst_ss, float* scales, int64_t scale_sp, float* wave_max) {
   constexpr int UPR = D / 16;   // units per row
   const PagedCache& c = p.c;
   const int nt = blockDim.x, tid = threadIdx.x;
-  if ((int)blockIdx.x >= store_blocks) {
-    const int64_t unit = (int64_t)((int)blockIdx.x - store_blocks) * nt + tid;
-    const int u = (int)(unit % UPR);
-    const int64_t row = unit / UPR;
-    if (row >= (int64_t)c.total * c.Hq) return;
-    const int t = (int)(row / c.Hq), h = (int)(row % c.Hq);
-    int b, i;
-    const bool in = token_place(c, t, b, i);
-    const int64_t pos = in ? (int64_t)max(c.seqlens[b], 0) + i : c.capacity;
-    T* out = (T*)p.q_out + (c.cu ? t * p.qo_ss : b * p.qo_sb + i * p.qo_ss) + h * p.qo_sh;
-    if (pos >= c.capacity) {   // outside every sequence, or past the table
-      st_u4(out + u * 16, u32x4{0, 0, 0, 0});
-      st_u4(out + u * 16 + 8, u32x4{0, 0, 0, 0});
-      return;
-    }
-    const T* in_row = (const T*)p.q + (c.cu ? t * p.q_ss : b * p.q_sb + i * p.q_ss) + h * p.q_sh;
-    int ca, cb;
-    float y[16];
-    load_unit(in_row, u, p.rotary, p.interleaved, p.cos + pos * p.cos_ss, p.sin + pos * p.sin_ss, ca, cb, y);
-    put_chunk(out, ca, y);
-    put_chunk(out, cb, y + 8);
-    return;
-  }
-
-  __shared__ float wave_max[4];
-  const int h = blockIdx.x % c.Hkv;
-  int rest = blockIdx.x / c.Hkv;
-  const bool is_v = rest & 1;
-  rest >>= 1;
-  const int b = rest / p.pages_per_seq;
   int off, len;
   token_range(c, b, off, len);
   const int L = max(c.seqlens[b], 0);
   const int64_t end = min((int64_t)L + len, (int64_t)c.capacity);   // rows after the append
-  const T* src = is_v ? (const T*)p.v + (c.cu ? off * p.v_ss : b * p.v_sb) + h * p.v_sh
-                      : (const T*)p.k + (c.cu ? off * p.k_ss : b * p.k_sb) + h * p.k_sh;
-  const int64_t src_ss = is_v ? p.v_ss : p.k_ss;
-  const int64_t dst_ss = is_v ? c.v_ss : c.k_ss;
-  const int rotary = is_v ? 0 : p.rotary;
-  for (int64_t page = L / c.page_size + rest % p.pages_per_seq; page * c.page_size < end; page += p.pages_per_seq) {
+  if (c.cu) src += off * src_ss;
+  for (int64_t page = L / c.page_size + first_page; page * c.page_size < end; page += p.pages_per_seq) {
     const int pid = c.table[b * c.table_sb + page];
     if (pid < 0 || pid >= c.num_pages) continue;
     const int64_t first = page * c.page_size;
     const int r0 = (int)(max((int64_t)L, first) - first);                // first new row of the page
     const int rows = (int)(min(end, first + c.page_size) - first) - r0;
     if (rows <= 0) continue;
-    const int i0 = (int)(first + r0 - L);                                // its token
+    const int64_t i0 = first + r0 - L;                                   // its token
     const int total = rows * UPR;
-    auto load = [&](int e, int& r, int& ca, int& cb, float (&y)[16]) {
-      r = e / UPR;
+    uint8_t* base = cache + pid * dst_sp;
+    float* sp = scales + pid * scale_sp;
+    const float old = r0 > 0 ? *sp : 0.f;   // filled from its first row on: the old scale is another sequence's
+    auto load = [&](int e, float (&y)[16]) {
+      const int r = e / UPR, u = e % UPR;
+      int ca, cb;
+      unit_chunks<MODE>(u, p.rotary, ca, cb);
+      const T* row = src + (i0 + r) * src_ss;
       const int64_t pos = first + r0 + r;
-      load_unit(src + (int64_t)(i0 + r) * src_ss, e % UPR, rotary, p.interleaved, p.cos + pos * p.cos_ss,
-                p.sin + pos * p.sin_ss, ca, cb, y);
+      const vec8<T> a = ld8(row + ca * 8), b8 = ld8(row + cb * 8);
+      const Angles t = unit_angles<MODE>(u, p.rotary, p.cos + pos * p.cos_ss, p.sin + pos * p.sin_ss);
+      rotate_unit<MODE, T, D>(a, b8, u, p.rotary, t, y);
     };
-    if constexpr (!FP8) {
-      T* dst = (is_v ? (T*)c.v + pid * c.v_sp + h * c.v_sh : (T*)c.k + pid * c.k_sp + h * c.k_sh) + r0 * dst_ss;
-      for (int e = tid; e < total; e += nt) {
-        int r, ca, cb;
-        float y[16];
-        load(e, r, ca, cb, y);
-        put_chunk(dst + r * dst_ss, ca, y);
-        put_chunk(dst + r * dst_ss, cb, y + 8);
+    auto store = [&](int e, const float (&y)[16], float inv) {
+      const int r = e / UPR, u = e % UPR;
+      int ca, cb;
+      unit_chunks<MODE>(u, p.rotary, ca, cb);
+      uint8_t* row = base + (r0 + r) * dst_ss;
+      put_codes(row, ca, y, inv);
+      put_codes(row, cb, y + 8, inv);
+    };
+    float held[kAppendHold][16];
+    float amax = 0.f;   // (fmaxf passes over NaN)
+#pragma unroll
+    for (int q = 0; q < kAppendHold; ++q) {
+      const int e = tid + q * nt;
+      if (e < total) {
+        load(e, held[q]);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(held[q][j]));
       }
-    } else {
-      uint8_t* base = is_v ? (uint8_t*)c.v + pid * c.v_sp + h * c.v_sh : (uint8_t*)c.k + pid * c.k_sp + h * c.k_sh;
-      uint8_t* dst = base + r0 * dst_ss;
-      float* sp = is_v ? c.v_scale + pid * c.vs_sp + h * c.vs_sh : c.k_scale + pid * c.ks_sp + h * c.ks_sh;
-      const float old = r0 > 0 ? *sp : 0.f;   // filled from its first row on: the old scale is another sequence's
-      float held[kAppendHold][16];
-      float amax = 0.f;
+    }
+    for (int e = tid + kAppendHold * nt; e < total; e += nt) {
+      float y[16];
+      load(e, y);
 #pragma unroll
-      for (int q = 0; q < kAppendHold; ++q) {
-        const int e = tid + q * nt;
-        if (e < total) {
-          int r, ca, cb;
-          load(e, r, ca, cb, held[q]);
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(y[j]));
+    }
+    auto of_all = [&](float x) {   // the largest of the workgroup's threads
 #pragma unroll
-          for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(held[q][j]));
-        }
-      }
-      for (int e = tid + kAppendHold * nt; e < total; e += nt) {
-        int r, ca, cb;
-        float y[16];
-        load(e, r, ca, cb, y);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(y[j]));
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-      __syncthreads();   // wave_max of the previous page has been read
-      if ((tid & 63) == 0) wave_max[tid >> 6] = amax;
+      for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+      __syncthreads();   // what wave_max held has been read
+      if ((tid & 63) == 0) wave_max[tid >> 6] = x;
       __syncthreads();
-      for (int w = 0; w < (nt + 63) / 64; ++w) amax = fmaxf(amax, wave_max[w]);
-      const float scale = fmaxf(old, page_scale(amax));   // (an old NaN counts as none)
-      const float inv = 1.f / scale;
-      if (tid == 0) *sp = scale;
-      if (r0 > 0 && scale > old) {   // the rows before the new ones, in the new units
-        const float ratio = old * inv;
-        for (int e = tid; e < r0 * (D / 16); e += nt) {
-          u32x4* at = reinterpret_cast<u32x4*>(base + (int64_t)(e / (D / 16)) * dst_ss + (e % (D / 16)) * 16);
-          u32x4 x = *at;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float y[4];
-            e4m3_unpack4(x[j], y);
-            x[j] = e4m3_pack4(y[0] * ratio, y[1] * ratio, y[2] * ratio, y[3] * ratio);
-          }
-          *at = x;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < kAppendHold; ++q) {
-        const int e = tid + q * nt;
-        if (e < total) {
-          const int u = e % UPR;
-          const bool halves = u * 16 < rotary && !p.interleaved;
-          uint8_t* row = dst + (int64_t)(e / UPR) * dst_ss;
-          put_chunk8(row, halves ? u : 2 * u, held[q], inv);
-          put_chunk8(row, halves ? u + rotary / 16 : 2 * u + 1, held[q] + 8, inv);
-        }
-      }
-      for (int e = tid + kAppendHold * nt; e < total; e += nt) {
-        int r, ca, cb;
+      for (int w = 0; w < (nt + 63) / 64; ++w) x = fmaxf(x, wave_max[w]);
+      return x;
+    };
+    amax = of_all(amax);
+    const bool infinite = amax == INFINITY;
+    if (infinite) {   // once more, of the finite ones
+      amax = 0.f;
+      for (int e = tid; e < total; e += nt) {
         float y[16];
-        load(e, r, ca, cb, y);
-        put_chunk8(dst + r * dst_ss, ca, y, inv);
-        put_chunk8(dst + r * dst_ss, cb, y + 8, inv);
+        load(e, y);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(y[j]) < INFINITY ? fabsf(y[j]) : 0.f);
       }
+      amax = of_all(amax);
+    }
+    const float scale = fmaxf(old, page_scale(amax));   // (an old NaN counts as none)
+    const float inv = 1.f / scale;
+    if (tid == 0) *sp = scale;
+    if (r0 > 0 && scale > old) {   // the rows before the new ones, in the new units
+      const float ratio = old * inv;
+      for (int e = tid; e < r0 * UPR; e += nt) {
+        u32x4* at = reinterpret_cast<u32x4*>(base + (int64_t)(e / UPR) * dst_ss + (e % UPR) * 16);
+        u32x4 x = *at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y[4];
+          e4m3_unpack4(x[j], y);
+          x[j] = e4m3_pack4(y[0] * ratio, y[1] * ratio, y[2] * ratio, y[3] * ratio);
+        }
+        *at = x;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kAppendHold; ++q) {
+      const int e = tid + q * nt;
+      if (e < total) {
+        if (infinite) scale_saturated(held[q], inv);
+        store(e, held[q], infinite ? 1.f : inv);
+      }
+    }
+    for (int e = tid + kAppendHold * nt; e < total; e += nt) {
+      float y[16];
+      load(e, y);
+      if (infinite) scale_saturated(y, inv);
+      store(e, y, infinite ? 1.f : inv);
     }
   }
 }
 
+// Blocks below `page_blocks` write codes, the others rows.
 template <class T, bool FP8, int D>
-static hipError_t launch_append_t(const PagedAppendParams& p, hipStream_t st) {
+__global__ void __launch_bounds__(kAppendThreads)
+paged_append_kernel(PagedAppendParams p, int page_blocks) {
   const PagedCache& c = p.c;
-  // threads: a page's new rows in one unit each, up to four waves
+  if ((int)blockIdx.x >= page_blocks) {
+    append_rows<T, D>(p, (int64_t)((int)blockIdx.x - page_blocks) * blockDim.x + threadIdx.x);
+    return;
+  }
+  if constexpr (FP8) {
+    __shared__ float wave_max[kAppendThreads / 64];
+    const int h = blockIdx.x % c.Hkv;
+    int rest = blockIdx.x / c.Hkv;
+    const bool is_v = rest & 1;
+    rest >>= 1;
+    const int b = rest / p.pages_per_seq, first = rest % p.pages_per_seq;
+    if (is_v) {
+      append_codes<kNoRotation, T, D>(p, b, h, first, (const T*)p.v + (c.cu ? 0 : b * p.v_sb) + h * p.v_sh, p.v_ss,
+                                      (uint8_t*)c.v + h * c.v_sh, c.v_sp, c.v_ss, c.v_scale + h * c.vs_sh, c.vs_sp, wave_max);
+      return;
+    }
+    const T* k = (const T*)p.k + (c.cu ? 0 : b * p.k_sb) + h * p.k_sh;
+    uint8_t* to = (uint8_t*)c.k + h * c.k_sh;
+    float* sc = c.k_scale + h * c.ks_sh;
+    if (!p.rotary) append_codes<kNoRotation, T, D>(p, b, h, first, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
+    else if (p.interleaved) append_codes<kInterleaved, T, D>(p, b, h, first, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
+    else append_codes<kHalves, T, D>(p, b, h, first, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
+  }
+}
+
+template <class T, bool FP8, int D>
+static hipError_t launch_append_t(const PagedAppendParams& pin, hipStream_t st) {
+  PagedAppendParams p = pin;
+  const PagedCache& c = p.c;
+  p.row_groups = (p.q ? cdiv(c.Hq, kRowHeads) : 0) + (FP8 ? 0 : 2 * cdiv(c.Hkv, kRowHeads));
+  // threads: a page's new rows in kAppendHold units each, or a wave's worth of units
   const int rows = c.n < c.page_size ? c.n : c.page_size;
-  int nt = (rows * (D / 16) + 63) / 64 * 64;
-  nt = nt > 256 ? 256 : nt;
-  const int64_t store = (int64_t)c.B * p.pages_per_seq * 2 * c.Hkv;
-  const int64_t query = p.q ? ((int64_t)c.total * c.Hq * (D / 16) + nt - 1) / nt : 0;
-  if (store + query > 0x7fffffff) return hipErrorInvalidValue;
-  if (store + query == 0) return hipSuccess;
-  hipLaunchKernelGGL((paged_append_kernel<T, FP8, D>), dim3((unsigned)(store + query)), dim3(nt), 0, st, p, (int)store);
+  int nt = FP8 ? (rows * (D / 16) + 64 * kAppendHold - 1) / (64 * kAppendHold) * 64 : 256;
+  nt = nt > kAppendThreads ? kAppendThreads : nt < 64 ? 64 : nt;
+  const int64_t pages = FP8 ? (int64_t)c.B * p.pages_per_seq * 2 * c.Hkv : 0;
+  const int64_t items = (int64_t)c.total * p.row_groups * (D / 16);
+  const int64_t blocks = pages + (items + nt - 1) / nt;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  if (blocks == 0) return hipSuccess;
+  hipLaunchKernelGGL((paged_append_kernel<T, FP8, D>), dim3((unsigned)blocks), dim3(nt), 0, st, p, (int)pages);
   return hipGetLastError();
 }
 
