@@ -968,7 +968,7 @@ PagedPlan plan_of(const fal_paged_cache& c) {
   // bytes that a head's row has for itself: a whole page where heads lie one after the other
   const bool by_row = c.heads_kv > 1 && c.k_strides[1] < c.k_strides[2];
   const int64_t row_bytes = (c.fp8 ? 1 : 2) * c.head_dim * (by_row ? 1 : c.page_size);
-  return paged_plan(c.batch, c.seqlen, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim, c.fp8 != 0, c.cu_seqlens != nullptr,
+  return paged_plan(c.batch, c.seqlen, c.total_tokens, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim, c.fp8 != 0, c.cu_seqlens != nullptr,
                     (int)std::min<int64_t>(row_bytes, 1 << 20), std::max(device_cu_count(), 1));
 }
 

@@ -264,7 +264,7 @@ hipError_t launch_decode(const DecodeParams& p, int d, hipStream_t st);
 hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st);
 hipError_t launch_paged_attn(const PagedAttnParams& p, int d, hipStream_t st);
 // row_bytes: bytes next to each other that belong to one KV head
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
                      int row_bytes, int ncu);
 
 }  // namespace fal

@@ -7,6 +7,7 @@
 // relative precision wherever its scale puts it, multiplying by the scale is exact, and when a
 // later token raises a page's scale the older codes keep their mantissas (only what falls
 // below e4m3's smallest normal is rounded again).
+#include <algorithm>
 #include <type_traits>
 
 #include "fal_kernels.h"
@@ -599,6 +600,11 @@ paged_split_kernel(PagedAttnParams p) {
 
   constexpr int CB = FP8 ? 1 : 2;
   const int k_ss = (int)c.k_ss * CB, v_ss = (int)c.v_ss * CB;   // row strides in bytes (below 2^23)
+  const char* const kbase = (const char*)c.k + hkv * c.k_sh * CB;
+  const char* const vbase = (const char*)c.v + hkv * c.v_sh * CB;
+  const uint32_t k_page = (uint32_t)(c.k_sp * CB >> 4), v_page = (uint32_t)(c.v_sp * CB >> 4);   // 16-byte units
+  const float* const kscale = FP8 ? c.k_scale + hkv * c.ks_sh : nullptr;
+  const float* const vscale = FP8 ? c.v_scale + hkv * c.vs_sh : nullptr;
   // K: 16 bytes g4 of row l16 in piece t, or, by lines, of row l16 % 8 (+ 8 in the second of a
   // pair) and piece t + l16 / 8 (kline order; see unswap)
   const int kv0 = l16 * k_ss + g4 * 16;
@@ -619,7 +625,7 @@ paged_split_kernel(PagedAttnParams p) {
   constexpr int VROW = VS::RB;
   const int kk = l16 >> 1;                                   // e4m3: row kk of the 8, slice kk / 4
   const int vr = FP8 ? 4 * g4 + (kk & 3) : 4 * g4 + (l16 >> 2);
-  const uint8_t* vbase = FP8 ? ring + (kk >> 2) * VS::BYTES + vr * VROW + 8 * (l16 & 1) : ring + vr * VROW + 8 * (l16 & 1);
+  const uint8_t* vread = FP8 ? ring + (kk >> 2) * VS::BYTES + vr * VROW + 8 * (l16 & 1) : ring + vr * VROW + 8 * (l16 & 1);
   const int vc0 = FP8 ? VS::swz(vr, kk >> 2) : ((l16 >> 1) & 1) ^ VS::swz(vr, 0);
 
   for (; left > 0; ++b, local = 0) {
@@ -676,11 +682,11 @@ paged_split_kernel(PagedAttnParams p) {
         const int pid = c.table[b * c.table_sb + page];
         if (pid >= 0 && pid < c.num_pages) {
           nrow = min(16, k_end - r);
-          koff = (pid * c.k_sp + hkv * c.k_sh + slot * c.k_ss) * CB;
-          voff = (pid * c.v_sp + hkv * c.v_sh + slot * c.v_ss) * CB;
+          koff = ((uint64_t)(uint32_t)pid * k_page << 4) + (uint32_t)(slot * k_ss);
+          voff = ((uint64_t)(uint32_t)pid * v_page << 4) + (uint32_t)(slot * v_ss);
           if (FP8) {
-            ksc = c.k_scale[pid * c.ks_sp + hkv * c.ks_sh];
-            vsc = c.v_scale[pid * c.vs_sp + hkv * c.vs_sh];
+            ksc = kscale[(uint64_t)(uint32_t)pid * (uint32_t)c.ks_sp];
+            vsc = vscale[(uint64_t)(uint32_t)pid * (uint32_t)c.vs_sp];
           }
         }
       }
@@ -692,8 +698,8 @@ paged_split_kernel(PagedAttnParams p) {
         const int n = (int)lane_of((uint32_t)nrow, i);
         const int64_t ko = (int64_t)(((uint64_t)lane_of((uint32_t)(koff >> 32), i) << 32) | lane_of((uint32_t)koff, i));
         const int64_t vo = (int64_t)(((uint64_t)lane_of((uint32_t)(voff >> 32), i) << 32) | lane_of((uint32_t)voff, i));
-        const auto krs = make_rsrc((const char*)c.k + ko, n > 0 ? (uint32_t)((n - 1) * k_ss + D * CB) : 0);
-        const auto vrs = make_rsrc((const char*)c.v + vo, n > 0 ? (uint32_t)((n - 1) * v_ss + D * CB) : 0);
+        const auto krs = make_rsrc(kbase + ko, n > 0 ? (uint32_t)((n - 1) * k_ss + D * CB) : 0);
+        const auto vrs = make_rsrc(vbase + vo, n > 0 ? (uint32_t)((n - 1) * v_ss + D * CB) : 0);
   #pragma unroll
         for (int t = 0; t < KL; ++t) {
           const bool pair = LINE && (t | 1) < KL;
@@ -796,10 +802,10 @@ paged_split_kernel(PagedAttnParams p) {
       for (int db = 0; db < DBN; ++db) {
         V8 vop;
         if constexpr (FP8) {
-          const u32x2 x = lds_tr8(vbase + buf * 2 * VS::BYTES + ((db ^ vc0) << 4));
+          const u32x2 x = lds_tr8(vread + buf * 2 * VS::BYTES + ((db ^ vc0) << 4));
           vop = e4m3_to_16<T>(x[0], x[1]);
         } else {
-          const T* v0 = (const T*)(vbase + buf * 2 * VS::BYTES + ((vc0 ^ (2 * db)) << 4));
+          const T* v0 = (const T*)(vread + buf * 2 * VS::BYTES + ((vc0 ^ (2 * db)) << 4));
           vop = join8(lds_tr(v0), lds_tr((const T*)((const uint8_t*)v0 + VS::BYTES)));
         }
 #pragma unroll
@@ -902,6 +908,17 @@ paged_split_kernel(PagedAttnParams p) {
 // * Scales as in the split kernel: the value factor enters the exponent, and each slice's sum is
 //   divided by it again for l.
 constexpr int kTileCols = 128;
+// Tiles in LDS: swizzled rows, or for head dim 96 rows padded to 208 bytes, of which any sixteen
+// start on different 16-byte pieces of the 256 that the banks hold.
+template <int D>
+struct PagedTile : SwizzledTile<D> {
+  static constexpr int LD = D;
+};
+template <>
+struct PagedTile<96> {
+  static constexpr int LD = 104;
+  __device__ static int offset(int r, int c) { return r * LD + c * 8; }
+};
 constexpr int tile_rows(int d) { return d > 128 ? 32 : 64; }   // (head dim 256: registers)
 
 template <class T, bool FP8, int D>
@@ -914,8 +931,8 @@ paged_tile_kernel(PagedAttnParams p) {
   constexpr int LOADS = (RW * CPR + 63) / 64;                // pieces per lane of those
   constexpr int CB = FP8 ? 1 : 2;
   using V8 = vec8<T>;
-  using Tile = SwizzledTile<D>;
-  __shared__ __attribute__((aligned(1024))) T ksm[2][TR * D], vsm[2][TR * D];
+  using Tile = PagedTile<D>;
+  __shared__ __attribute__((aligned(1024))) T ksm[2][TR * Tile::LD], vsm[2][TR * Tile::LD];
   __shared__ float ssm[2][NS][2];                             // per slice: key and value scale (-1: no page)
 
   const PagedCache& c = p.c;
@@ -1370,6 +1387,9 @@ paged_merge_kernel(PagedAttnParams p) {
   if (p.lse && d == 0) p.lse[row] = sum > 0.f ? (M + fast_log2(sum)) * kLn2 : -INFINITY;
 }
 
+#ifndef FAL_PAGED_TILE_OVER
+#define FAL_PAGED_TILE_OVER 1
+#endif
 #ifndef FAL_PAGED_TILE_FROM
 #define FAL_PAGED_TILE_FROM 32
 #endif
@@ -1385,7 +1405,7 @@ paged_merge_kernel(PagedAttnParams p) {
 #ifndef FAL_PAGED_DIRECT
 #define FAL_PAGED_DIRECT 2048
 #endif
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
                      int row_bytes, int ncu) {
   PagedPlan r{};
   r.max_cols = FAL_PAGED_TILE_FROM;
@@ -1393,9 +1413,11 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t Hq, int64_t Hkv, int64_t
   if (wide > r.max_cols) {
     const int64_t tiles = (wide + kTileCols - 1) / kTileCols;
     r.tile_cols = (int)tiles;
-    const int64_t blocks = B * Hkv * tiles, slots = (int64_t)ncu * (d > 128 ? 1 : 2);
+    // column tiles of packed tokens: at most one that is not full in each sequence
+    const int64_t all = std::min(B * tiles, total * (Hq / Hkv) / kTileCols + B);
+    const int64_t blocks = Hkv * all, slots = (int64_t)ncu * (d > 128 ? 1 : 2) * FAL_PAGED_TILE_OVER;
     const int64_t longest = (capacity + 4 * tile_rows(d) - 1) / (4 * tile_rows(d));   // (four tiles at least)
-    int64_t n = slots / (blocks > 0 ? blocks : 1);
+    int64_t n = (slots + blocks / 2) / (blocks > 0 ? blocks : 1);
     n = n > 16 ? 16 : n > longest ? longest : n;
     r.splits = (int)(n < 1 ? 1 : n);
     return r;
