@@ -994,7 +994,7 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   const PagedPlan plan = plan_of(c);
   p.parts = plan.parts, p.unit_rows = plan.unit_rows, p.wave_heads = plan.wave_heads;
   p.nc = plan.nc, p.col_tiles = plan.col_tiles, p.cols = plan.cols, p.direct = plan.direct;
-  p.splits = plan.splits, p.tile_cols = plan.tile_cols;
+  p.splits = plan.splits, p.tile_cols = plan.tile_cols, p.row_split = plan.row_split;
   const size_t rows = paged_partials(plan, c);
   p.part_o = static_cast<float*>(workspace);
   p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(rows * c.head_dim * sizeof(float)));

@@ -191,13 +191,13 @@ struct PagedAttnParams {
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
   // tile kernel (splits > 0): tile_cols column tiles of the longest sequence, each sequence's rows
   // in `splits` shares; tile_blocks workgroups, and rest_blocks for packed rows outside every sequence
-  int splits, tile_cols, tile_blocks, rest_blocks;
+  int splits, tile_cols, row_split, tile_blocks, rest_blocks;   // row_split: waves that share a column's rows
   float* part_o;      // [parts + B, Hkv, cols, d], or [total, Hq, splits, d]
   float* part_m;      // the same without d: log2-domain LSE
 };
 struct PagedPlan {
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
-  int splits, tile_cols, max_cols;
+  int splits, tile_cols, row_split, max_cols;
 };
 
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);

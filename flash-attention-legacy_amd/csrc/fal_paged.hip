@@ -895,7 +895,8 @@ paged_split_kernel(PagedAttnParams p) {
 // ---------------------------------------------------------------------------
 // Attention, many columns: tiles of keys shared by a workgroup
 // ---------------------------------------------------------------------------
-// One workgroup takes 128 columns (see above) of one sequence and KV head, 32 to a wave, and
+// One workgroup takes 128 columns (see above) of one sequence and KV head, 32 to a wave (or 64, and
+// two waves share a column's rows: half of the matrix units would idle otherwise), and
 // walks tiles of 64 or 32 rows; with few workgroups, `splits` of them share a column tile's rows.
 // * Each wave brings a slice of the tile (16 rows of one page, or half of one) from the cache: its
 //   page and scales are scalars, its lanes' places in the page constants, and e4m3 codes become 16-bit values
@@ -908,6 +909,9 @@ paged_split_kernel(PagedAttnParams p) {
 // * Scales as in the split kernel: the value factor enters the exponent, and each slice's sum is
 //   divided by it again for l.
 constexpr int kTileCols = 128;
+#ifndef FAL_PAGED_AHEAD
+#define FAL_PAGED_AHEAD(d, fp8) ((d) <= ((fp8) ? 128 : 64) ? 2 : 1)
+#endif
 // Tiles in LDS: swizzled rows, or for head dim 96 rows padded to 208 bytes, of which any sixteen
 // start on different 16-byte pieces of the 256 that the banks hold.
 template <int D>
@@ -921,17 +925,19 @@ struct PagedTile<96> {
 };
 constexpr int tile_rows(int d) { return d > 128 ? 32 : 64; }   // (head dim 256: registers)
 
-template <class T, bool FP8, int D>
+template <class T, bool FP8, int D, int RS>
 __global__ void __launch_bounds__(256, D > 128 ? 1 : 2)
 paged_tile_kernel(PagedAttnParams p) {
   constexpr int DB = D / 32, KS = D / 16;
   constexpr int RB = FP8 ? D : 2 * D, CPR = RB / 16;         // bytes of a cache row, its 16-byte pieces
-  constexpr int TR = tile_rows(D), NS = TR / 16;             // rows and slices of a tile
+  constexpr int TR = tile_rows(D), NS = TR / 16, NW = NS / RS;   // rows and slices of a tile, slices of a wave
   constexpr int RW = TR / 4;                                 // rows that a wave brings
   constexpr int LOADS = (RW * CPR + 63) / 64;                // pieces per lane of those
   constexpr int CB = FP8 ? 1 : 2;
+  constexpr int AHEAD = FAL_PAGED_AHEAD(D, FP8);
   using V8 = vec8<T>;
   using Tile = PagedTile<D>;
+  constexpr int TC = kTileCols / RS;                         // columns of a tile
   __shared__ __attribute__((aligned(1024))) T ksm[2][TR * Tile::LD], vsm[2][TR * Tile::LD];
   __shared__ float ssm[2][NS][2];                             // per slice: key and value scale (-1: no page)
 
@@ -966,17 +972,18 @@ paged_tile_kernel(PagedAttnParams p) {
   const int step_pages = TR / c.page_size, step_rows = TR - step_pages * c.page_size;
   // column tiles, those that see the most rows first; past the stated longest sequence each
   // workgroup takes further ones
-  for (int ct = p.tile_cols - 1 - rest / p.splits; ct * kTileCols < ncols; ct += p.tile_cols) {
-    const int col_last = min(ncols, (ct + 1) * kTileCols) - 1;
+  for (int ct = p.tile_cols - 1 - rest / p.splits; ct * TC < ncols; ct += p.tile_cols) {
+    const int col_last = min(ncols, (ct + 1) * TC) - 1;
     const int k_hi = max(p.causal ? L - len + col_last / G + 1 : L, 0);
     const int tiles = cdiv(k_hi, TR);
     const int t0 = (int)((int64_t)tiles * split / p.splits), t1 = (int)((int64_t)tiles * (split + 1) / p.splits);
 
     // this wave's columns
-    const int col = ct * kTileCols + w * 32 + l32, i_tok = col / G, head = hkv * G + col % G;
-    const bool have = col < ncols, active = ct * kTileCols + w * 32 < ncols;
+    const int wc = w % (4 / RS), wx = w / (4 / RS) * NW;     // its 32 columns and its first slice
+    const int col = ct * TC + wc * 32 + l32, i_tok = col / G, head = hkv * G + col % G;
+    const bool have = col < ncols, active = ct * TC + wc * 32 < ncols;
     const int lim = p.causal ? L - len + i_tok + 1 : L;
-    const int lim_first = p.causal ? L - len + (ct * kTileCols + w * 32) / G + 1 : L;
+    const int lim_first = p.causal ? L - len + (ct * TC + wc * 32) / G + 1 : L;
     V8 qreg[KS];
     const T* qrow = (const T*)p.q + (c.cu ? (int64_t)(off + i_tok) * p.q_ss : b * p.q_sb + i_tok * p.q_ss) + head * p.q_sh;
 #pragma unroll
@@ -1012,9 +1019,10 @@ paged_tile_kernel(PagedAttnParams p) {
       if (slot >= c.page_size) slot -= c.page_size, ++page;
       return x;
     };
-    u32x4 kreg[LOADS], vreg[LOADS];
-    float ksc = 1.f, vsc = 1.f;
-    auto fetch = [&](Slice x) {
+    u32x4 kreg[AHEAD][LOADS], vreg[AHEAD][LOADS];
+    float ksc[AHEAD], vsc[AHEAD];
+    auto fetch = [&](auto slotc, Slice x) {
+      constexpr int at = decltype(slotc)::value;
       const uint32_t pid = x.pid >= 0 ? x.pid : 0;
       const auto krs = make_rsrc(kbase + ((uint64_t)pid * k_page << 4) + (uint32_t)(x.slot * k_ss),
                                  x.rows > 0 ? (uint32_t)((x.rows - 1) * k_ss + RB) : 0);
@@ -1022,16 +1030,17 @@ paged_tile_kernel(PagedAttnParams p) {
                                  x.rows > 0 ? (uint32_t)((x.rows - 1) * v_ss + RB) : 0);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        kreg[i] = __builtin_amdgcn_raw_buffer_load_b128(krs, kv[i], 0, 0);
-        vreg[i] = __builtin_amdgcn_raw_buffer_load_b128(vrs, vv[i], 0, 0);
+        kreg[at][i] = __builtin_amdgcn_raw_buffer_load_b128(krs, kv[i], 0, 0);
+        vreg[at][i] = __builtin_amdgcn_raw_buffer_load_b128(vrs, vv[i], 0, 0);
       }
-      vsc = x.rows > 0 ? 1.f : -1.f;
+      ksc[at] = 1.f, vsc[at] = x.rows > 0 ? 1.f : -1.f;
       if (FP8 && x.rows > 0) {
-        ksc = kscale[(uint64_t)pid * (uint32_t)c.ks_sp];
-        vsc = vscale[(uint64_t)pid * (uint32_t)c.vs_sp];
+        ksc[at] = kscale[(uint64_t)pid * (uint32_t)c.ks_sp];
+        vsc[at] = vscale[(uint64_t)pid * (uint32_t)c.vs_sp];
       }
     };
-    auto stage = [&](int buf) {
+    auto stage = [&](auto slotc, int buf) {
+      constexpr int at = decltype(slotc)::value;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int e = i * 64 + lane, r = e / CPR, u = e % CPR, row = w * RW + r;
@@ -1039,40 +1048,47 @@ paged_tile_kernel(PagedAttnParams p) {
         if constexpr (FP8) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            st_u4(&ksm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(kreg[i][2 * x], kreg[i][2 * x + 1])));
-            st_u4(&vsm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(vreg[i][2 * x], vreg[i][2 * x + 1])));
+            st_u4(&ksm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(kreg[at][i][2 * x], kreg[at][i][2 * x + 1])));
+            st_u4(&vsm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(vreg[at][i][2 * x], vreg[at][i][2 * x + 1])));
           }
         } else {
-          st_u4(&ksm[buf][Tile::offset(row, u)], kreg[i]);
-          st_u4(&vsm[buf][Tile::offset(row, u)], vreg[i]);
+          st_u4(&ksm[buf][Tile::offset(row, u)], kreg[at][i]);
+          st_u4(&vsm[buf][Tile::offset(row, u)], vreg[at][i]);
         }
       }
-      if (lane == 0 && w * RW % 16 == 0) ssm[buf][w * RW / 16][0] = ksc, ssm[buf][w * RW / 16][1] = vsc;
+      if (lane == 0 && w * RW % 16 == 0) ssm[buf][w * RW / 16][0] = ksc[at], ssm[buf][w * RW / 16][1] = vsc[at];
     };
 
     if (t0 < t1) {
+      // tile n waits in registers n % AHEAD; tile t + 1 is staged while t is computed
+      const std::integral_constant<int, 0> r0;
+      const std::integral_constant<int, AHEAD - 1> r1;
       const Slice s0 = next_slice(), s1 = next_slice();
+      fetch(r0, s0);
+      if constexpr (AHEAD == 2) fetch(r1, s1);
       Slice coming = next_slice();
-      fetch(s0);
-      stage(0);
-      fetch(s1);
+      stage(r0, 0);
+      fetch(r0, AHEAD == 2 ? coming : s1);
+      if constexpr (AHEAD == 2) coming = next_slice();
       __syncthreads();
       auto step = [&](auto bufc, int t) {
         constexpr int buf = decltype(bufc)::value;
         if (active) {
           // S^T: element i of block mb is row mb * 32 + (i / 4) * 8 + hh * 4 + i % 4, column l32
-          constexpr int MB = TR / 32;
+          constexpr int MB = TR / 32 / RS;
+          const T* const kt = &ksm[buf][wx * 16 * Tile::LD];
+          const T* const vt = &vsm[buf][wx * 16 * Tile::LD];
           f32x16 s[MB];
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) s[mb] = zero_f16();
-          constexpr int KB = 2;   // k-steps whose operands are read together, one group ahead
+          constexpr int KB = AHEAD == 2 && D == 128 ? 1 : 2;   // k-steps whose operands are read together, one group ahead
           V8 ka[2][MB][KB];
           auto read_k = [&](int g) {
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
               for (int i = 0; i < KB; ++i)
-                ka[g & 1][mb][i] = ld8(&ksm[buf][Tile::offset(mb * 32 + l32, (g * KB + i) * 2 + hh)]);
+                ka[g & 1][mb][i] = ld8(kt + Tile::offset(mb * 32 + l32, (g * KB + i) * 2 + hh));
           };
           read_k(0);
 #pragma unroll
@@ -1093,21 +1109,21 @@ paged_tile_kernel(PagedAttnParams p) {
 #pragma unroll
             for (int i = 0; i < VG; ++i) {
               const int ch = (g % VH * VG + i) * 4 + tc;
-              va[g & 1][i] = join8(lds_tr(&vsm[buf][Tile::offset(x * 16 + tr, ch) + (lane & 1) * 4]),
-                                   lds_tr(&vsm[buf][Tile::offset(x * 16 + 8 + tr, ch) + (lane & 1) * 4]));
+              va[g & 1][i] = join8(lds_tr(vt + Tile::offset(x * 16 + tr, ch) + (lane & 1) * 4),
+                                   lds_tr(vt + Tile::offset(x * 16 + 8 + tr, ch) + (lane & 1) * 4));
             }
           };
           read_v(0);
           __builtin_amdgcn_sched_barrier(0);
-          // slice x: elements 8 (x % 2) .. + 8 of block x / 2
-          float kfac[NS], vlog[NS], vinv[NS], back = 1.f;
+          // the wave's slice x: elements 8 (x % 2) .. + 8 of block x / 2
+          float kfac[NW], vlog[NW], vinv[NW], back = 1.f;
           bool whole = (t + 1) * TR <= lim_first;
           if constexpr (FP8) {
-            float v[NS], now = ref;
+            float v[NW], now = ref;
 #pragma unroll
-            for (int x = 0; x < NS; ++x) {
-              kfac[x] = fmaxf(p.scale_log2 * ssm[buf][x][0], 0x1p-126f);
-              v[x] = ssm[buf][x][1];
+            for (int x = 0; x < NW; ++x) {
+              kfac[x] = fmaxf(p.scale_log2 * ssm[buf][wx + x][0], 0x1p-126f);
+              v[x] = ssm[buf][wx + x][1];
               whole = whole && __builtin_amdgcn_readfirstlane(__float_as_int(v[x])) >= 0;
               now = fmaxf(now, v[x]);
             }
@@ -1115,31 +1131,31 @@ paged_tile_kernel(PagedAttnParams p) {
             back = ref * inv;
             ref = now;
 #pragma unroll
-            for (int x = 0; x < NS; ++x) {   // (a value scale 2^60 below the largest counts as that)
+            for (int x = 0; x < NW; ++x) {   // (a value scale 2^60 below the largest counts as that)
               const float f = fmaxf(v[x] * inv, 0x1p-60f);
               vlog[x] = fast_log2(f), vinv[x] = __builtin_amdgcn_rcpf(f);
             }
           } else {
 #pragma unroll
-            for (int x = 0; x < NS; ++x) {
+            for (int x = 0; x < NW; ++x) {
               kfac[x] = p.scale_log2, vlog[x] = 0.f, vinv[x] = 1.f;
-              whole = whole && __builtin_amdgcn_readfirstlane(__float_as_int(ssm[buf][x][1])) >= 0;
+              whole = whole && __builtin_amdgcn_readfirstlane(__float_as_int(ssm[buf][wx + x][1])) >= 0;
             }
           }
           if (!whole) {
 #pragma unroll
-            for (int x = 0; x < NS; ++x) {
-              const bool none = ssm[buf][x][1] < 0.f;
+            for (int x = 0; x < NW; ++x) {
+              const bool none = ssm[buf][wx + x][1] < 0.f;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const int r = t * TR + x * 16 + (i / 4) * 8 + hh * 4 + i % 4;
+                const int r = t * TR + (wx + x) * 16 + (i / 4) * 8 + hh * 4 + i % 4;
                 if (none || r >= lim) s[x / 2][(x & 1) * 8 + i] = -INFINITY;
               }
             }
           }
           float mx = -INFINITY;
 #pragma unroll
-          for (int x = 0; x < NS; ++x) {
+          for (int x = 0; x < NW; ++x) {
             const f32x16& y = s[x / 2];
             const int o = (x & 1) * 8;
             float a = y[o];
@@ -1158,9 +1174,9 @@ paged_tile_kernel(PagedAttnParams p) {
             for (int i = 0; i < DB; ++i) oacc[i] *= f;
           }
           const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-          V8 pb[NS];
+          V8 pb[NW];
 #pragma unroll
-          for (int x = 0; x < NS; ++x) {
+          for (int x = 0; x < NW; ++x) {
             const float sub = FP8 ? vlog[x] - m_use : -m_use;
             float l = 0.f;
 #pragma unroll
@@ -1173,8 +1189,8 @@ paged_tile_kernel(PagedAttnParams p) {
           }
           // O^T += V^T P^T
 #pragma unroll
-          for (int g = 0; g < NS * VH; ++g) {
-            if (g + 1 < NS * VH) read_v(g + 1);
+          for (int g = 0; g < NW * VH; ++g) {
+            if (g + 1 < NW * VH) read_v(g + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < VG; ++i)
@@ -1182,8 +1198,9 @@ paged_tile_kernel(PagedAttnParams p) {
           }
         }
         if (t + 1 < t1) {
-          stage(buf ^ 1);
-          fetch(coming);
+          const std::integral_constant<int, (buf ^ 1) % AHEAD> r;
+          stage(r, buf ^ 1);
+          fetch(r, coming);
           coming = next_slice();
         }
         __syncthreads();
@@ -1195,8 +1212,38 @@ paged_tile_kernel(PagedAttnParams p) {
       }
     }
 
-    if (have) {
-      l_run = pair_sum(l_run);
+    l_run = pair_sum(l_run);
+    if constexpr (RS == 2) {   // the two waves of a column meet: the second one's sums go through LDS
+      float* const mls = reinterpret_cast<float*>(&vsm[0][0]) + wc * 128;
+      f32x4* const sums = reinterpret_cast<f32x4*>(&ksm[0][0]) + wc * (DB * 4 * 64);
+      static_assert(sizeof(ksm) >= 2 * DB * 4 * 64 * sizeof(f32x4), "two waves' sums fit");
+      if (wx) {
+        mls[lane] = m_ref, mls[64 + lane] = l_run;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float f = FP8 ? ref : 1.f;
+            sums[(db * 4 + i) * 64 + lane] =
+                f32x4{oacc[db][4 * i], oacc[db][4 * i + 1], oacc[db][4 * i + 2], oacc[db][4 * i + 3]} * f;
+          }
+      }
+      __syncthreads();
+      if (!wx) {
+        const float m2 = mls[lane], m = fmaxf(m_ref, m2), use = m == -INFINITY ? 0.f : m;
+        const float a1 = fast_exp2(m_ref - use), a2 = fast_exp2(m2 - use);
+        m_ref = m;
+        l_run = l_run * a1 + mls[64 + lane] * a2;
+        const float f = a1 * (FP8 ? ref : 1.f);
+        ref = 1.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) oacc[db][i] = oacc[db][i] * f + sums[(db * 4 + i / 4) * 64 + lane][i % 4] * a2;
+      }
+      __syncthreads();   // before the next columns' tiles are staged
+    }
+    if (have && !wx) {
       const float f = l_run > 0.f ? (FP8 ? ref : 1.f) / l_run : 0.f;
       const float lse2 = l_run > 0.f ? m_ref + fast_log2(l_run) : -INFINITY;
       const int64_t row = (int64_t)((c.cu ? off : b * c.n) + i_tok) * c.Hq + head;
@@ -1265,18 +1312,22 @@ __device__ void attend_alone(const PagedAttnParams& p, int b, int i, int h, cons
   }
 }
 
-// One workgroup of four waves per (token, query head): merge the pieces' partial outputs.  Each
-// wave takes every fourth piece, eight of them in flight, with weights relative to its own
-// largest LSE, and the four sums meet in LDS in a fixed order.
-template <class T, bool FP8, int D>
+// Merge the pieces' partial outputs of (token, query head) rows, W waves to a row and four waves
+// to a workgroup.  Each wave takes every W-th piece, eight of them in flight, with weights
+// relative to its own largest LSE; four waves of a row meet in LDS in a fixed order.  (One wave
+// for rows of few pieces: 10240 rows of about four, 34 -> COMB1 us.)
+template <class T, bool FP8, int D, int W>
 __global__ void __launch_bounds__(256)
 paged_combine_kernel(PagedAttnParams p) {
   constexpr int DJ = (D + 63) / 64;
   constexpr int CH = 8;
   __shared__ float m_s[4], l_s[4], o_s[4][D];
   const PagedCache& c = p.c;
-  const int h = blockIdx.x % c.Hq, t = blockIdx.x / c.Hq;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * (4 / W) + (W == 4 ? 0 : wave);
+  if (row >= (int64_t)c.total * c.Hq) return;
+  const int w = W == 4 ? wave : 0;
+  const int h = (int)(row % c.Hq), t = (int)(row / c.Hq);
   int b = 0, i = 0, ns = 0;
   const bool in = token_place(c, t, b, i);
   const bool alone = in && i >= c.n;   // past the stated longest sequence
@@ -1302,20 +1353,19 @@ paged_combine_kernel(PagedAttnParams p) {
       base = ((int64_t)(g0 + b) * c.Hkv + h / G) * p.cols + i * G + h % G;
     }
   }
-  const int64_t row = (int64_t)t * c.Hq + h;
   float acc[DJ];
 #pragma unroll
   for (int j = 0; j < DJ; ++j) acc[j] = 0.f;
   float M = -INFINITY, wsum = 0.f;
-  for (int s0 = w; s0 < ns; s0 += 4 * CH) {
+  for (int s0 = w; s0 < ns; s0 += W * CH) {
     float pm[CH], x[CH][DJ];
 #pragma unroll
     for (int u = 0; u < CH; ++u) {
-      const bool ok = s0 + 4 * u < ns;
-      pm[u] = ok ? p.part_m[base + (s0 + 4 * u) * step] : -INFINITY;
-      const float* po = p.part_o + (base + (s0 + 4 * u) * step) * D;
+      const bool ok = s0 + W * u < ns;
+      const int64_t at = base + (s0 + W * u) * step;
+      pm[u] = ok ? p.part_m[at] : -INFINITY;
 #pragma unroll
-      for (int j = 0; j < DJ; ++j) x[u][j] = (ok && lane + 64 * j < D) ? po[lane + 64 * j] : 0.f;
+      for (int j = 0; j < DJ; ++j) x[u][j] = (ok && lane + 64 * j < D) ? p.part_o[at * D + lane + 64 * j] : 0.f;
     }
     float cm = -INFINITY;
 #pragma unroll
@@ -1337,23 +1387,31 @@ paged_combine_kernel(PagedAttnParams p) {
   }
   if (alone && w == 0)
     attend_alone<T, FP8, D>(p, b, i, h, (const T*)p.q + t * p.q_ss + h * p.q_sh, acc, M, wsum);
-  if (lane == 0) m_s[w] = M, l_s[w] = wsum;
-#pragma unroll
-  for (int j = 0; j < DJ; ++j)
-    if (lane + 64 * j < D) o_s[w][lane + 64 * j] = acc[j];
-  __syncthreads();
-  const float top = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-  float f[4], sum = 0.f;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    f[u] = m_s[u] == -INFINITY ? 0.f : fast_exp2(m_s[u] - top);
-    sum += l_s[u] * f[u];
-  }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
   T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
-  for (int d = threadIdx.x; d < D; d += 256)
-    orow[d] = (T)((o_s[0][d] * f[0] + o_s[1][d] * f[1] + o_s[2][d] * f[2] + o_s[3][d] * f[3]) * inv);
-  if (p.lse && threadIdx.x == 0) p.lse[row] = sum > 0.f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
+  if constexpr (W == 1) {
+    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+#pragma unroll
+    for (int j = 0; j < DJ; ++j)
+      if (lane + 64 * j < D) orow[lane + 64 * j] = (T)(acc[j] * inv);
+    if (p.lse && lane == 0) p.lse[row] = wsum > 0.f ? (M + fast_log2(wsum)) * kLn2 : -INFINITY;
+  } else {
+    if (lane == 0) m_s[w] = M, l_s[w] = wsum;
+#pragma unroll
+    for (int j = 0; j < DJ; ++j)
+      if (lane + 64 * j < D) o_s[w][lane + 64 * j] = acc[j];
+    __syncthreads();
+    const float top = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
+    float f[4], sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f[u] = m_s[u] == -INFINITY ? 0.f : fast_exp2(m_s[u] - top);
+      sum += l_s[u] * f[u];
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    for (int d = threadIdx.x; d < D; d += 256)
+      orow[d] = (T)((o_s[0][d] * f[0] + o_s[1][d] * f[1] + o_s[2][d] * f[2] + o_s[3][d] * f[3]) * inv);
+    if (p.lse && threadIdx.x == 0) p.lse[row] = sum > 0.f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
+  }
 }
 
 // Merge the tile kernel's splits, four elements of one (token, query head) per thread.
@@ -1411,10 +1469,11 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64
   r.max_cols = FAL_PAGED_TILE_FROM;
   const int64_t wide = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
   if (wide > r.max_cols) {
-    const int64_t tiles = (wide + kTileCols - 1) / kTileCols;
+    r.row_split = wide <= kTileCols / 2 && d <= 128 ? 2 : 1;
+    const int64_t tile_cols = kTileCols / r.row_split, tiles = (wide + tile_cols - 1) / tile_cols;
     r.tile_cols = (int)tiles;
     // column tiles of packed tokens: at most one that is not full in each sequence
-    const int64_t all = std::min(B * tiles, total * (Hq / Hkv) / kTileCols + B);
+    const int64_t all = std::min(B * tiles, total * (Hq / Hkv) / tile_cols + B);
     const int64_t blocks = Hkv * all, slots = (int64_t)ncu * (d > 128 ? 1 : 2) * FAL_PAGED_TILE_OVER;
     const int64_t longest = (capacity + 4 * tile_rows(d) - 1) / (4 * tile_rows(d));   // (four tiles at least)
     int64_t n = (slots + blocks / 2) / (blocks > 0 ? blocks : 1);
@@ -1441,8 +1500,9 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64
 template <class T, bool FP8, int D>
 static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
   if (p.splits) {
-    hipLaunchKernelGGL((paged_tile_kernel<T, FP8, D>), dim3((unsigned)(p.tile_blocks + (p.splits > 1 ? 0 : p.rest_blocks))),
-                       dim3(256), 0, st, p);
+    const dim3 tiles((unsigned)(p.tile_blocks + (p.splits > 1 ? 0 : p.rest_blocks)));
+    if (D > 128 || p.row_split == 1) hipLaunchKernelGGL((paged_tile_kernel<T, FP8, D, 1>), tiles, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_tile_kernel<T, FP8, (D > 128 ? 128 : D), 2>), tiles, dim3(256), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t threads = (int64_t)p.c.total * p.c.Hq * (D / 4);
@@ -1454,7 +1514,11 @@ static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
   else hipLaunchKernelGGL((paged_split_kernel<T, FP8, (D > 128 ? 128 : D), 2>), grid, block, 0, st, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.direct) return e;
-  hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D>), dim3((unsigned)(p.c.total * p.c.Hq)), dim3(256), 0, st, p);
+  const int64_t rows = (int64_t)p.c.total * p.c.Hq;
+  if (p.parts / p.c.B < 8)   // (pieces of a sequence, about)
+    hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
