@@ -1487,8 +1487,10 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64
   r.col_tiles = (int)((cols + 16 * r.nc - 1) / (16 * r.nc));
   r.cols = r.col_tiles * 16 * r.nc;
   r.wave_heads = 1;
-  r.direct = capacity <= FAL_PAGED_DIRECT && !packed;
-  while (!r.direct && r.wave_heads < FAL_PAGED_WH && Hkv % (2 * r.wave_heads) == 0) r.wave_heads *= 2;
+  r.direct = capacity <= FAL_PAGED_DIRECT && !packed && B * Hkv * r.col_tiles <= ncu;
+  // rows of a run with one, two, four heads to a workgroup: HEADRULE
+  const int64_t run_rows = B * capacity * Hkv / ncu;
+  if (!r.direct && Hkv % 2 == 0 && run_rows >= 2 * 1280) r.wave_heads = Hkv % 4 == 0 && run_rows >= 4 * 2048 ? 4 : 2;
   r.unit_rows = FAL_PAGED_UNIT * waves / r.wave_heads;
   const int64_t most = B * ((capacity + r.unit_rows - 1) / r.unit_rows + 1);
   int64_t parts = (int64_t)ncu * FAL_PAGED_WPC / (Hkv / r.wave_heads * r.col_tiles);
