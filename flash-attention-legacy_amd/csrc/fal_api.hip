@@ -823,13 +823,16 @@ int check_cache(const char* name, const fal_paged_cache& c, const void* p, const
     if (st[i] < 0 || st[i] > (int64_t(1) << 33) || st[i] * bytes % 16 != 0)
       return fail(FAL_ERR_INVALID, "%s: stride[%d]=%lld must be a non-negative multiple of 16 bytes up to 2^33", name, i,
                   (long long)st[i]);
-  // kernels address the rows of a page with 32-bit byte offsets
+  // kernels address the rows of a page with 32-bit byte offsets, and 16 of them at once
   if (st[2] >= (int64_t(1) << 22))
     return fail(FAL_ERR_UNSUPPORTED, "%s: row stride %lld elements is too large (limit 4194304)", name,
                 (long long)st[2]);
   if (st[2] < c.head_dim)
     return fail(FAL_ERR_UNSUPPORTED, "%s: row stride %lld is shorter than a row of %lld elements", name,
                 (long long)st[2], (long long)c.head_dim);
+  if (c.page_size * st[2] * bytes > 0x7fffffff)
+    return fail(FAL_ERR_UNSUPPORTED, "%s: a page of %lld rows %lld elements apart passes 2^31 bytes", name,
+                (long long)c.page_size, (long long)st[2]);
   if (!written) return FAL_OK;
   // no two rows of a cache that is written may share memory: in the order of their strides,
   // each axis steps over all that the ones before it span
@@ -860,6 +863,9 @@ int check_scale(const char* name, const fal_paged_cache& c, const float* p, cons
     return fail(FAL_ERR_INVALID, "%s: entries overlap", name);
   return FAL_OK;
 }
+
+// The longest sequence's tokens, as the caller has it
+int64_t stated_longest(const fal_paged_cache& c) { return c.cu_seqlens ? std::min(c.seqlen, c.total_tokens) : c.seqlen; }
 
 // What both calls share: sizes, page table, token ranges and caches.
 int fill_paged(PagedCache& p, const fal_paged_cache* cache, int bf16, bool written) {
@@ -896,7 +902,7 @@ int fill_paged(PagedCache& p, const fal_paged_cache* cache, int bf16, bool writt
   p.v_sp = c.v_strides[0], p.v_sh = c.v_strides[1], p.v_ss = c.v_strides[2];
   p.ks_sp = c.k_scale_strides[0], p.ks_sh = c.k_scale_strides[1];
   p.vs_sp = c.v_scale_strides[0], p.vs_sh = c.v_scale_strides[1];
-  p.B = (int)c.batch, p.n = (int)c.seqlen, p.total = (int)c.total_tokens;
+  p.B = (int)c.batch, p.n = (int)stated_longest(c), p.total = (int)c.total_tokens;
   p.Hq = (int)c.heads_q, p.Hkv = (int)c.heads_kv;
   p.num_pages = (int)c.num_pages, p.page_size = (int)c.page_size, p.capacity = (int)(c.max_pages * c.page_size);
   p.fp8 = c.fp8 != 0, p.bf16 = bf16;
@@ -951,7 +957,7 @@ int paged_append_impl(const fal_paged_cache* cache, const void* k, const void* v
   }
   p.rotary = (int)rotary_dim, p.interleaved = rotary_interleaved != 0;
   // pages that seqlen rows can touch
-  p.pages_per_seq = (int)((std::max<int64_t>(c.seqlen, 1) + c.page_size - 2) / c.page_size + 1);
+  p.pages_per_seq = (int)((std::max<int64_t>(p.c.n, 1) + c.page_size - 2) / c.page_size + 1);
   if (c.batch * p.pages_per_seq > 0x7fffffff / (2 * c.heads_kv) ||
       c.batch * p.pages_per_seq * 2 * c.heads_kv + c.total_tokens * c.heads_q * c.head_dim / 16 / 64 >= 0x7fffffff)
     return fail(FAL_ERR_INVALID, "problem too large for one launch");
@@ -965,11 +971,8 @@ size_t paged_partials(const PagedPlan& plan, const fal_paged_cache& c) {
 }
 
 PagedPlan plan_of(const fal_paged_cache& c) {
-  // bytes that a head's row has for itself: a whole page where heads lie one after the other
-  const bool by_row = c.heads_kv > 1 && c.k_strides[1] < c.k_strides[2];
-  const int64_t row_bytes = (c.fp8 ? 1 : 2) * c.head_dim * (by_row ? 1 : c.page_size);
-  return paged_plan(c.batch, c.seqlen, c.total_tokens, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim, c.fp8 != 0, c.cu_seqlens != nullptr,
-                    (int)std::min<int64_t>(row_bytes, 1 << 20), std::max(device_cu_count(), 1));
+  return paged_plan(c.batch, stated_longest(c), c.total_tokens, c.heads_q, c.heads_kv, c.max_pages * c.page_size, (int)c.head_dim,
+                    c.fp8 != 0, c.cu_seqlens != nullptr, std::max(device_cu_count(), 1));
 }
 
 int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float* lse, const int64_t* q_strides,
@@ -998,7 +1001,7 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   const size_t rows = paged_partials(plan, c);
   p.part_o = static_cast<float*>(workspace);
   p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(rows * c.head_dim * sizeof(float)));
-  if (c.total_tokens * c.heads_q > 0x7fffffff || c.seqlen * c.heads_q > 0x7fffffff)
+  if (c.total_tokens * c.heads_q > 0x7fffffff)
     return fail(FAL_ERR_INVALID, "problem too large for one launch");
   if (plan.splits) {
     const int64_t per = (int64_t)plan.splits * c.heads_kv * plan.tile_cols;

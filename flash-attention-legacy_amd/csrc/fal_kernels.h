@@ -197,7 +197,7 @@ struct PagedAttnParams {
 };
 struct PagedPlan {
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
-  int splits, tile_cols, row_split, max_cols;
+  int splits, tile_cols, row_split;
 };
 
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);
@@ -263,8 +263,7 @@ hipError_t launch_decode(const DecodeParams& p, int d, hipStream_t st);
 
 hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st);
 hipError_t launch_paged_attn(const PagedAttnParams& p, int d, hipStream_t st);
-// row_bytes: bytes next to each other that belong to one KV head
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
-                     int row_bytes, int ncu);
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64_t Hkv, int64_t capacity, int d,
+                     bool fp8, bool packed, int ncu);
 
 }  // namespace fal

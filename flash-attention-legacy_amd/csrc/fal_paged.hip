@@ -429,6 +429,12 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return pair_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
 }
 
+// log2-domain LSE of a sum of weights relative to m: -infinity if no row was seen, NaN if one of
+// the scores was.
+__device__ __forceinline__ float lse_of(float m, float sum) { return sum == 0.f ? -INFINITY : m + fast_log2(sum); }
+// In a partial result infinity stands for NaN, which a maximum would pass over.
+__device__ __forceinline__ float partial_lse(float lse2) { return lse2 != lse2 ? INFINITY : lse2; }
+
 // Eight e4m3 codes as 16-bit values (exact)
 template <class T>
 __device__ __forceinline__ vec8<T> e4m3_to_16(uint32_t lo, uint32_t hi) {
@@ -520,18 +526,91 @@ __device__ __forceinline__ int lanes_scan(int x) {
   return x;
 }
 
-// Units of 64 sequences, one per lane, and their inclusive sums.  The first unit of a sequence
-// has no rows: it stands for what starting and ending one costs (page table, scales, first rows,
-// merge: about as long as UNITUS of streaming), so that runs that cross into the next sequence
-// get fewer rows and all end together.
-__device__ __forceinline__ int lane_units(const PagedCache& c, int base, int unit_rows, int lane, int& sum) {
-  const int rows = base + lane < c.B ? cache_rows(c, base + lane) : 0;
-  const int u = rows > 0 ? cdiv(rows, unit_rows) + 1 : 0;
-  sum = lanes_scan(u);
-  return u;
+// Units of the sequences, by blocks of 64, one sequence per lane; four blocks are read at once, so
+// that large batches cost one round trip to memory in 256.  The first unit of a sequence has no
+// rows: it stands for what starting and ending one costs (page table, scales, first rows, merge),
+// so that runs that cross into the next sequence get fewer rows and all end together (24
+// sequences of 77 to 4099 rows in 21 runs per head: 37.3 -> 35.3 us).
+constexpr int kBlocks = 4;
+struct UnitBlocks {
+  int unit[kBlocks], sum[kBlocks];   // a lane's units, and the inclusive sums within its block
+  __device__ UnitBlocks(const PagedCache& c, int base, int unit_rows, int lane) {
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+      const int b = base + 64 * k + lane;
+      const int rows = b < c.B ? cache_rows(c, b) : 0;
+      unit[k] = rows > 0 ? cdiv(rows, unit_rows) + 1 : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) sum[k] = base + 64 * k < c.B ? lanes_scan(unit[k]) : 0;
+  }
+  __device__ int total(int k) const { return (int)lane_of((uint32_t)sum[k], 63); }
+  __device__ int before(int k, int at) const { return (int)(lane_of((uint32_t)sum[k], at) - lane_of((uint32_t)unit[k], at)); }
+};
+
+// Rows r0 .. r1 of the attention of one token i and query head h of sequence b, by one wave, row
+// after row: the sums o of weights relative to m times values (element lane + 64 j in o[j]), and
+// the weights' sum l.  For what the matrix kernels leave out: tokens past the stated longest
+// sequence, and columns whose result is not finite under a causal mask, since in a matrix product
+// a value that is not finite makes the columns that do not see its row NaN too (0 * infinity).
+template <class T, bool FP8, int D>
+__device__ void attend_alone(const PagedAttnParams& p, int b, int i, int h, int r0, int r1, float (&o)[(D + 63) / 64],
+                             float& m, float& l) {
+  const PagedCache& c = p.c;
+  constexpr int DJ = (D + 63) / 64, CB = FP8 ? 1 : 2;
+  const int lane = threadIdx.x & 63, hk = h / (c.Hq / c.Hkv);
+  auto elem = [&](const char* row, int e) {
+    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[e], 0);
+    else return (float)((const T*)row)[e];
+  };
+  int off, len;
+  token_range(c, b, off, len);
+  const T* qrow = (const T*)p.q + (c.cu ? (int64_t)(off + i) * p.q_ss : b * p.q_sb + i * p.q_ss) + h * p.q_sh;
+  float q[DJ];
+#pragma unroll
+  for (int j = 0; j < DJ; ++j) {
+    const int e = lane + 64 * j;
+    q[j] = e < D ? (float)qrow[e] * (p.negate_q ? -p.scale_log2 : p.scale_log2) : 0.f;
+    o[j] = 0.f;
+  }
+  const int L = cache_rows(c, b), end = min(p.causal ? L - len + i + 1 : L, r1);
+  m = -INFINITY, l = 0.f;
+  for (int r = r0; r < end; ++r) {
+    const int pid = c.table[b * c.table_sb + r / c.page_size], slot = r % c.page_size;
+    if (pid < 0 || pid >= c.num_pages) continue;
+    const char* k = (const char*)c.k + (pid * c.k_sp + hk * c.k_sh + slot * c.k_ss) * CB;
+    const char* v = (const char*)c.v + (pid * c.v_sp + hk * c.v_sh + slot * c.v_ss) * CB;
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < DJ; ++j)
+      if (lane + 64 * j < D) x = fmaf(q[j], elem(k, lane + 64 * j), x);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+    if (FP8) x *= c.k_scale[pid * c.ks_sp + hk * c.ks_sh];
+    const float mn = fmaxf(m, x), use = mn == -INFINITY ? 0.f : mn;
+    const float a = fast_exp2(m - use), e = fast_exp2(x - use);
+    m = mn;
+    l = l * a + e;
+    const float ev = FP8 ? e * c.v_scale[pid * c.vs_sp + hk * c.vs_sh] : e;
+#pragma unroll
+    for (int j = 0; j < DJ; ++j)
+      if (lane + 64 * j < D) o[j] = fmaf(ev, elem(v, lane + 64 * j), o[j] * a);
+  }
 }
 
-template <class T, bool FP8, int D, int NC>
+// NaN if one of the values is not finite, else 0
+template <int N, class Acc>
+__device__ __forceinline__ float not_finite(const Acc (&x)[N]) {
+  float bad = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Acc) / sizeof(float)); ++i) bad = fmaf(x[k][i], 0.f, bad);
+  return bad;
+}
+
+// ONE: one token per sequence, which sees every row (sequences with more are the combine kernel's).
+template <class T, bool FP8, int D, int NC, bool ONE>
 __global__ void __launch_bounds__(paged_waves(D, FP8) * 64, paged_waves(D, FP8) / 4)
 paged_split_kernel(PagedAttnParams p) {
   constexpr int NW = paged_waves(D, FP8);
@@ -540,10 +619,7 @@ paged_split_kernel(PagedAttnParams p) {
   using VS = VSlice<FP8, D>;
   // K registers of a slice: 16-byte pieces that cover 64 bytes of each of its 16 rows
   constexpr int KL = FP8 ? D / 64 : D / 32, KTAIL = FP8 ? (D % 64) / 32 : 0;   // (tail: 32 bytes of each row)
-#ifndef FAL_PAGED_LINE
-#define FAL_PAGED_LINE 1
-#endif
-  constexpr bool LINE = KL >= 2 && FAL_PAGED_LINE;   // pairs of pieces loaded as whole 128-byte lines
+  constexpr bool LINE = KL >= 2;                 // pairs of pieces loaded as whole 128-byte lines
   constexpr int LPS = 2 * (KL + KTAIL + VS::LOADS);
   using V8 = vec8<T>;
   __shared__ __attribute__((aligned(1024))) uint8_t vsm[NW][4 * VS::BYTES];   // 2 steps x 2 slices
@@ -572,27 +648,31 @@ paged_split_kernel(PagedAttnParams p) {
   if (p.direct) {        // one run is one sequence
     b = run, left = 0x7fffffff;
   } else {
-    int sum, u = 0;
     int64_t units = 0;
-    for (int base = 0; base < c.B; base += 64) {
-      u = lane_units(c, base, p.unit_rows, lane, sum);
-      units += (int)lane_of((uint32_t)sum, 63);
+    for (int base = 0; base < c.B; base += 64 * kBlocks) {
+      const UnitBlocks x(c, base, p.unit_rows, lane);
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) units += x.total(k);
     }
     const Runs runs(units, p.parts);
     const int64_t u0 = runs.begin(run);
     left = __builtin_amdgcn_readfirstlane((int)(runs.begin(run + 1) - u0));
     if (left <= 0) return;
     int64_t before = 0;
-    for (int base = 0; base < c.B; base += 64) {
-      if (c.B > 64) u = lane_units(c, base, p.unit_rows, lane, sum);
-      const auto past = __ballot(before + sum > u0);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        b = base + at;
-        local = (int)(u0 - before) - (int)(lane_of((uint32_t)sum, at) - lane_of((uint32_t)u, at));
-        break;
+    bool found = false;
+    for (int base = 0; base < c.B && !found; base += 64 * kBlocks) {
+      const UnitBlocks x(c, base, p.unit_rows, lane);
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const auto past = __ballot(before + x.sum[k] > u0);
+        if (!found && past) {
+          const int at = __builtin_ctzll(past);
+          b = base + 64 * k + at;
+          local = (int)(u0 - before) - x.before(k, at);
+          found = true;
+        }
+        before += x.total(k);
       }
-      before += (int)lane_of((uint32_t)sum, 63);
     }
     b = __builtin_amdgcn_readfirstlane(b);
     local = __builtin_amdgcn_readfirstlane(local);
@@ -639,7 +719,7 @@ paged_split_kernel(PagedAttnParams p) {
     if ((row0 >= row1 && !p.direct) || ct * NC * 16 >= ncols) continue;
 
     // rows below this one are seen by every column
-    const int lim_first = p.causal ? L - len + ct * NC * 16 / G + 1 : L;
+    const int lim_first = !ONE && p.causal ? L - len + ct * NC * 16 / G + 1 : L;
     // queries of the columns as the B operand (n = column, k = head dim in K's order)
     V8 qreg[NC][KS];
     int lim[NC];         // rows below this one are seen by the column
@@ -648,7 +728,7 @@ paged_split_kernel(PagedAttnParams p) {
       const int col = (ct * NC + nc) * 16 + l16;
       const int i = col / G, h = hkv * G + col % G;
       const T* qrow = (const T*)p.q + (c.cu ? (int64_t)(off + i) * p.q_ss : b * p.q_sb + i * p.q_ss) + h * p.q_sh;
-      lim[nc] = p.causal ? L - len + i + 1 : L;
+      lim[nc] = !ONE && p.causal ? L - len + i + 1 : L;
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
         const int e = FP8 && t < 2 * KL ? (t >> 1) * 64 + g4 * 16 + (t & 1) * 8 : t * 32 + g4 * 8;
@@ -760,7 +840,7 @@ paged_split_kernel(PagedAttnParams p) {
         ref = now;
       }
       const int r0 = k_begin + j * 32;
-      const bool whole = n0 == 16 && n1 == 16 && r0 + 32 <= lim_first;   // every row seen by every column
+      const bool whole = n0 == 16 && n1 == 16 && (ONE || r0 + 32 <= lim_first);   // every row seen by every column
       V8 pb[NC];
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
@@ -770,7 +850,7 @@ paged_split_kernel(PagedAttnParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int r = 4 * g4 + i;
-              if (r >= (sl ? n1 : n0) || r0 + sl * 16 + r >= lim[nc]) s[nc][sl][i] = -INFINITY;
+              if (r >= (sl ? n1 : n0) || (!ONE && r0 + sl * 16 + r >= lim[nc])) s[nc][sl][i] = -INFINITY;
             }
         }
         float mx = fmaxf(fmaxf(fmaxf(s[nc][0][0], s[nc][0][1]), fmaxf(s[nc][0][2], s[nc][0][3])) * kfac[0],
@@ -835,20 +915,22 @@ paged_split_kernel(PagedAttnParams p) {
       *reinterpret_cast<vec4<T>*>((T*)p.o + b * p.o_sb + col / G * p.o_ss + (kv * G + col % G) * p.o_sh + d) = y;
     };
     auto put_lse = [&](int col, int kv, float lse2) {
-      if (!p.direct) p.part_m[(piece + kv) * p.cols + col] = lse2;
+      if (!p.direct) p.part_m[(piece + kv) * p.cols + col] = partial_lse(lse2);
       else if (p.lse) p.lse[((int64_t)b * c.n + col / G) * c.Hq + kv * G + col % G] = lse2 * kLn2;
     };
+    const bool masked = !ONE && p.causal && len > 1;
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       const int col0 = (ct * NC + nc) * 16;
       const int nh = min(16, ncols - col0);
-      const float l_tot = quarters_sum(l_run[nc]);
+      // (NaN marks a column whose result is not finite, which the combine kernel takes on)
+      const float l_tot = quarters_sum(masked ? l_run[nc] + not_finite(oacc[nc]) : l_run[nc]);
       if (NR == 1) {   // a wave has all of its head's rows
-        const float f = l_tot > 0.f ? (FP8 ? ref : 1.f) / l_tot : 0.f;
+        const float f = l_tot == 0.f ? 0.f : (FP8 ? ref : 1.f) / l_tot;
         if (l16 < nh) {
 #pragma unroll
           for (int db = 0; db < DBN; ++db) put(col0 + l16, hkv, db * 16 + 4 * g4, oacc[nc][db] * f);
-          if (g4 == 0) put_lse(col0 + l16, hkv, l_tot > 0.f ? m_run[nc] + fast_log2(l_tot) : -INFINITY);
+          if (g4 == 0) put_lse(col0 + l16, hkv, lse_of(m_run[nc], l_tot));
         }
         continue;
       }
@@ -873,8 +955,8 @@ paged_split_kernel(PagedAttnParams p) {
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) sum += i % WH == ws % WH ? lw[i] * fast_exp2(mw[i] - M_use) : 0.f;
-        inv_s[w][l16] = sum > 0.f ? 1.f / sum : 0.f;
-        put_lse(col0 + l16, hkv, sum > 0.f ? M_use + fast_log2(sum) : -INFINITY);
+        inv_s[w][l16] = sum == 0.f ? 0.f : 1.f / sum;
+        put_lse(col0 + l16, hkv, lse_of(M_use, sum));
       }
       __syncthreads();
       for (int k = 0; k < WH; ++k) {
@@ -909,9 +991,6 @@ paged_split_kernel(PagedAttnParams p) {
 // * Scales as in the split kernel: the value factor enters the exponent, and each slice's sum is
 //   divided by it again for l.
 constexpr int kTileCols = 128;
-#ifndef FAL_PAGED_AHEAD
-#define FAL_PAGED_AHEAD(d, fp8) ((d) <= ((fp8) ? 128 : 64) ? 2 : 1)
-#endif
 // Tiles in LDS: swizzled rows, or for head dim 96 rows padded to 208 bytes, of which any sixteen
 // start on different 16-byte pieces of the 256 that the banks hold.
 template <int D>
@@ -925,6 +1004,41 @@ struct PagedTile<96> {
 };
 constexpr int tile_rows(int d) { return d > 128 ? 32 : 64; }   // (head dim 256: registers)
 
+// The kernel's parameter block, read again where it is named: a path that is hardly ever taken
+// then keeps nothing of it in registers all the way (a kernel's first argument opens the segment).
+template <class P>
+__device__ __forceinline__ const P& args_again() {
+  auto a = (const __attribute__((address_space(4))) P*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *(const P*)a;
+}
+
+// Column `col` of sequence b and KV head hkv over the rows r0 .. r1 of a split, by one wave (see
+// attend_alone).  Not inlined: it is hardly ever reached, and inlined it took registers from the
+// loop (chunk of 1024 tokens behind 8192 rows: ALONE0).
+template <class T, bool FP8, int D>
+__device__ __attribute__((noinline)) void column_again(const PagedAttnParams& p, int b, int hkv, int col, int split, int r0, int r1) {
+  const PagedCache& c = p.c;
+  const int G = c.Hq / c.Hkv, i = col / G, h = hkv * G + col % G, lane = threadIdx.x & 63;
+  int off, len;
+  token_range(c, b, off, len);
+  float o[(D + 63) / 64], m, l;
+  attend_alone<T, FP8, D>(p, b, i, h, r0, r1, o, m, l);
+  const float inv = l == 0.f ? 0.f : 1.f / l, lse2 = lse_of(m, l);
+  const int64_t row = ((c.cu ? off : (int64_t)b * c.n) + i) * c.Hq + h;
+  T* orow = (T*)p.o + (c.cu ? (int64_t)(off + i) * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
+#pragma unroll
+  for (int j = 0; j < (D + 63) / 64; ++j) {
+    const int d = lane + 64 * j;
+    if (d >= D) continue;
+    if (p.splits > 1) p.part_o[(row * p.splits + split) * D + d] = o[j] * inv;
+    else orow[d] = (T)(o[j] * inv);
+  }
+  if (lane) return;
+  if (p.splits > 1) p.part_m[row * p.splits + split] = partial_lse(lse2);
+  else if (p.lse) p.lse[row] = lse2 * kLn2;
+}
+
 template <class T, bool FP8, int D, int RS>
 __global__ void __launch_bounds__(256, D > 128 ? 1 : 2)
 paged_tile_kernel(PagedAttnParams p) {
@@ -934,12 +1048,11 @@ paged_tile_kernel(PagedAttnParams p) {
   constexpr int RW = TR / 4;                                 // rows that a wave brings
   constexpr int LOADS = (RW * CPR + 63) / 64;                // pieces per lane of those
   constexpr int CB = FP8 ? 1 : 2;
-  constexpr int AHEAD = FAL_PAGED_AHEAD(D, FP8);
   using V8 = vec8<T>;
   using Tile = PagedTile<D>;
   constexpr int TC = kTileCols / RS;                         // columns of a tile
   __shared__ __attribute__((aligned(1024))) T ksm[2][TR * Tile::LD], vsm[2][TR * Tile::LD];
-  __shared__ float ssm[2][NS][2];                             // per slice: key and value scale (-1: no page)
+  __shared__ float ssm[2][NS][2];                            // per slice: key and value scale (-1: no page)
 
   const PagedCache& c = p.c;
   const int G = c.Hq / c.Hkv;
@@ -1019,10 +1132,9 @@ paged_tile_kernel(PagedAttnParams p) {
       if (slot >= c.page_size) slot -= c.page_size, ++page;
       return x;
     };
-    u32x4 kreg[AHEAD][LOADS], vreg[AHEAD][LOADS];
-    float ksc[AHEAD], vsc[AHEAD];
-    auto fetch = [&](auto slotc, Slice x) {
-      constexpr int at = decltype(slotc)::value;
+    u32x4 kreg[LOADS], vreg[LOADS];
+    float ksc, vsc;
+    auto fetch = [&](Slice x) {
       const uint32_t pid = x.pid >= 0 ? x.pid : 0;
       const auto krs = make_rsrc(kbase + ((uint64_t)pid * k_page << 4) + (uint32_t)(x.slot * k_ss),
                                  x.rows > 0 ? (uint32_t)((x.rows - 1) * k_ss + RB) : 0);
@@ -1030,17 +1142,16 @@ paged_tile_kernel(PagedAttnParams p) {
                                  x.rows > 0 ? (uint32_t)((x.rows - 1) * v_ss + RB) : 0);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        kreg[at][i] = __builtin_amdgcn_raw_buffer_load_b128(krs, kv[i], 0, 0);
-        vreg[at][i] = __builtin_amdgcn_raw_buffer_load_b128(vrs, vv[i], 0, 0);
+        kreg[i] = __builtin_amdgcn_raw_buffer_load_b128(krs, kv[i], 0, 0);
+        vreg[i] = __builtin_amdgcn_raw_buffer_load_b128(vrs, vv[i], 0, 0);
       }
-      ksc[at] = 1.f, vsc[at] = x.rows > 0 ? 1.f : -1.f;
+      ksc = 1.f, vsc = x.rows > 0 ? 1.f : -1.f;
       if (FP8 && x.rows > 0) {
-        ksc[at] = kscale[(uint64_t)pid * (uint32_t)c.ks_sp];
-        vsc[at] = vscale[(uint64_t)pid * (uint32_t)c.vs_sp];
+        ksc = kscale[(uint64_t)pid * (uint32_t)c.ks_sp];
+        vsc = vscale[(uint64_t)pid * (uint32_t)c.vs_sp];
       }
     };
-    auto stage = [&](auto slotc, int buf) {
-      constexpr int at = decltype(slotc)::value;
+    auto stage = [&](int buf) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int e = i * 64 + lane, r = e / CPR, u = e % CPR, row = w * RW + r;
@@ -1048,28 +1159,23 @@ paged_tile_kernel(PagedAttnParams p) {
         if constexpr (FP8) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            st_u4(&ksm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(kreg[at][i][2 * x], kreg[at][i][2 * x + 1])));
-            st_u4(&vsm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(vreg[at][i][2 * x], vreg[at][i][2 * x + 1])));
+            st_u4(&ksm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(kreg[i][2 * x], kreg[i][2 * x + 1])));
+            st_u4(&vsm[buf][Tile::offset(row, 2 * u + x)], __builtin_bit_cast(u32x4, e4m3_to_16<T>(vreg[i][2 * x], vreg[i][2 * x + 1])));
           }
         } else {
-          st_u4(&ksm[buf][Tile::offset(row, u)], kreg[at][i]);
-          st_u4(&vsm[buf][Tile::offset(row, u)], vreg[at][i]);
+          st_u4(&ksm[buf][Tile::offset(row, u)], kreg[i]);
+          st_u4(&vsm[buf][Tile::offset(row, u)], vreg[i]);
         }
       }
-      if (lane == 0 && w * RW % 16 == 0) ssm[buf][w * RW / 16][0] = ksc[at], ssm[buf][w * RW / 16][1] = vsc[at];
+      if (lane == 0 && w * RW % 16 == 0) ssm[buf][w * RW / 16][0] = ksc, ssm[buf][w * RW / 16][1] = vsc;
     };
 
     if (t0 < t1) {
-      // tile n waits in registers n % AHEAD; tile t + 1 is staged while t is computed
-      const std::integral_constant<int, 0> r0;
-      const std::integral_constant<int, AHEAD - 1> r1;
       const Slice s0 = next_slice(), s1 = next_slice();
-      fetch(r0, s0);
-      if constexpr (AHEAD == 2) fetch(r1, s1);
       Slice coming = next_slice();
-      stage(r0, 0);
-      fetch(r0, AHEAD == 2 ? coming : s1);
-      if constexpr (AHEAD == 2) coming = next_slice();
+      fetch(s0);
+      stage(0);
+      fetch(s1);
       __syncthreads();
       auto step = [&](auto bufc, int t) {
         constexpr int buf = decltype(bufc)::value;
@@ -1081,7 +1187,7 @@ paged_tile_kernel(PagedAttnParams p) {
           f32x16 s[MB];
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) s[mb] = zero_f16();
-          constexpr int KB = AHEAD == 2 && D == 128 ? 1 : 2;   // k-steps whose operands are read together, one group ahead
+          constexpr int KB = 2;   // k-steps whose operands are read together, one group ahead
           V8 ka[2][MB][KB];
           auto read_k = [&](int g) {
 #pragma unroll
@@ -1198,9 +1304,8 @@ paged_tile_kernel(PagedAttnParams p) {
           }
         }
         if (t + 1 < t1) {
-          const std::integral_constant<int, (buf ^ 1) % AHEAD> r;
-          stage(r, buf ^ 1);
-          fetch(r, coming);
+          stage(buf ^ 1);
+          fetch(coming);
           coming = next_slice();
         }
         __syncthreads();
@@ -1212,7 +1317,9 @@ paged_tile_kernel(PagedAttnParams p) {
       }
     }
 
-    l_run = pair_sum(l_run);
+    const bool masked = p.causal && len > 1;
+    // (NaN marks a column whose result is not finite)
+    l_run = pair_sum(masked ? l_run + not_finite(oacc) : l_run);
     if constexpr (RS == 2) {   // the two waves of a column meet: the second one's sums go through LDS
       float* const mls = reinterpret_cast<float*>(&vsm[0][0]) + wc * 128;
       f32x4* const sums = reinterpret_cast<f32x4*>(&ksm[0][0]) + wc * (DB * 4 * 64);
@@ -1243,10 +1350,12 @@ paged_tile_kernel(PagedAttnParams p) {
       }
       __syncthreads();   // before the next columns' tiles are staged
     }
-    if (have && !wx) {
-      const float f = l_run > 0.f ? (FP8 ? ref : 1.f) / l_run : 0.f;
-      const float lse2 = l_run > 0.f ? m_ref + fast_log2(l_run) : -INFINITY;
-      const int64_t row = (int64_t)((c.cu ? off : b * c.n) + i_tok) * c.Hq + head;
+    auto marked = __ballot(masked && have && !wx && hh == 0 && l_run != l_run);
+    const int64_t t_row = c.cu ? off : (int64_t)b * c.n;       // the sequence's first token
+    if (have && !wx && !(marked >> l32 & 1)) {
+      const float f = l_run == 0.f ? 0.f : (FP8 ? ref : 1.f) / l_run;
+      const float lse2 = lse_of(m_ref, l_run);
+      const int64_t row = (t_row + i_tok) * c.Hq + head;
       T* orow = (T*)p.o + (c.cu ? (int64_t)(off + i_tok) * p.o_ss : b * p.o_sb + i_tok * p.o_ss) + head * p.o_sh;
       float* part = p.part_o + (row * p.splits + split) * D;
 #pragma unroll
@@ -1259,56 +1368,12 @@ paged_tile_kernel(PagedAttnParams p) {
           else *reinterpret_cast<vec4<T>*>(orow + d) = vec4<T>{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
         }
       if (hh == 0) {
-        if (p.splits > 1) p.part_m[row * p.splits + split] = lse2;
+        if (p.splits > 1) p.part_m[row * p.splits + split] = partial_lse(lse2);
         else if (p.lse) p.lse[row] = lse2 * kLn2;
       }
     }
-  }
-}
-
-// Attention of one token i and query head h of sequence b by one wave, row after row: for tokens
-// past the stated longest sequence, which the grid of the split kernel has no columns for.
-template <class T, bool FP8, int D>
-__device__ void attend_alone(const PagedAttnParams& p, int b, int i, int h, const T* qrow, float (&o)[(D + 63) / 64],
-                             float& m, float& l) {
-  const PagedCache& c = p.c;
-  constexpr int DJ = (D + 63) / 64, CB = FP8 ? 1 : 2;
-  const int lane = threadIdx.x & 63, hk = h / (c.Hq / c.Hkv);
-  auto elem = [&](const char* row, int e) {
-    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[e], 0);
-    else return (float)((const T*)row)[e];
-  };
-  float q[DJ];
-#pragma unroll
-  for (int j = 0; j < DJ; ++j) {
-    const int e = lane + 64 * j;
-    q[j] = e < D ? (float)qrow[e] * (p.negate_q ? -p.scale_log2 : p.scale_log2) : 0.f;
-    o[j] = 0.f;
-  }
-  int off, len;
-  token_range(c, b, off, len);
-  const int L = cache_rows(c, b), end = p.causal ? L - len + i + 1 : L;
-  m = -INFINITY, l = 0.f;
-  for (int r = 0; r < end; ++r) {
-    const int pid = c.table[b * c.table_sb + r / c.page_size], slot = r % c.page_size;
-    if (pid < 0 || pid >= c.num_pages) continue;
-    const char* k = (const char*)c.k + (pid * c.k_sp + hk * c.k_sh + slot * c.k_ss) * CB;
-    const char* v = (const char*)c.v + (pid * c.v_sp + hk * c.v_sh + slot * c.v_ss) * CB;
-    float x = 0.f;
-#pragma unroll
-    for (int j = 0; j < DJ; ++j)
-      if (lane + 64 * j < D) x = fmaf(q[j], elem(k, lane + 64 * j), x);
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
-    if (FP8) x *= c.k_scale[pid * c.ks_sp + hk * c.ks_sh];
-    const float mn = fmaxf(m, x), use = mn == -INFINITY ? 0.f : mn;
-    const float a = fast_exp2(m - use), e = fast_exp2(x - use);
-    m = mn;
-    l = l * a + e;
-    const float ev = FP8 ? e * c.v_scale[pid * c.vs_sp + hk * c.vs_sh] : e;
-#pragma unroll
-    for (int j = 0; j < DJ; ++j)
-      if (lane + 64 * j < D) o[j] = fmaf(ev, elem(v, lane + 64 * j), o[j] * a);
+    for (; marked; marked &= marked - 1)
+      column_again<T, FP8, D>(args_again<PagedAttnParams>(), b, hkv, ct * TC + wc * 32 + __builtin_ctzll(marked), split, t0 * TR, t1 * TR);
   }
 }
 
@@ -1330,20 +1395,25 @@ paged_combine_kernel(PagedAttnParams p) {
   const int h = (int)(row % c.Hq), t = (int)(row / c.Hq);
   int b = 0, i = 0, ns = 0;
   const bool in = token_place(c, t, b, i);
-  const bool alone = in && i >= c.n;   // past the stated longest sequence
+  int off = 0, len = 1;
+  if (in) token_range(c, b, off, len);
+  const bool alone = in && (i >= c.n || (c.n == 1 && len > 1));   // past the stated longest sequence
   const int G = c.Hq / c.Hkv;
   int64_t base = 0, step = (int64_t)c.Hkv * p.cols;
   if (in && !alone) {   // this sequence's pieces
     int64_t units = 0, first = 0;
     int mine = 0;
-    for (int at = 0; at < c.B; at += 64) {
-      int sum;
-      const int u = lane_units(c, at, p.unit_rows, lane, sum);
-      if (b >= at && b < at + 64) {
-        mine = (int)lane_of((uint32_t)u, b - at);
-        first = units + (int)lane_of((uint32_t)sum, b - at) - mine;
+    for (int at = 0; at < c.B; at += 64 * kBlocks) {
+      const UnitBlocks x(c, at, p.unit_rows, lane);
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const int l = b - at - 64 * k;
+        if (l >= 0 && l < 64) {
+          first = units + x.before(k, l);
+          mine = (int)lane_of((uint32_t)x.unit[k], l);
+        }
+        units += x.total(k);
       }
-      units += (int)lane_of((uint32_t)sum, 63);
     }
     if (mine > 0) {
       const Runs runs(units, p.parts);
@@ -1385,15 +1455,25 @@ paged_combine_kernel(PagedAttnParams p) {
     }
     M = Mn;
   }
-  if (alone && w == 0)
-    attend_alone<T, FP8, D>(p, b, i, h, (const T*)p.q + t * p.q_ss + h * p.q_sh, acc, M, wsum);
+  // a piece that is not finite (see attend_alone): every wave of the row sees the same
+  bool again = false;
+  if (p.causal && c.n > 1)
+    for (int s0 = 0; s0 < ns; s0 += 64)
+      again = again || __any(s0 + lane < ns && p.part_m[base + (s0 + lane) * step] == INFINITY);
+  if (alone || again) {
+    if (w == 0) attend_alone<T, FP8, D>(p, b, i, h, 0, 0x7fffffff, acc, M, wsum);
+    else M = -INFINITY, wsum = 0.f;
+    if (w)
+#pragma unroll
+      for (int j = 0; j < DJ; ++j) acc[j] = 0.f;
+  }
   T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
   if constexpr (W == 1) {
-    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+    const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
 #pragma unroll
     for (int j = 0; j < DJ; ++j)
       if (lane + 64 * j < D) orow[lane + 64 * j] = (T)(acc[j] * inv);
-    if (p.lse && lane == 0) p.lse[row] = wsum > 0.f ? (M + fast_log2(wsum)) * kLn2 : -INFINITY;
+    if (p.lse && lane == 0) p.lse[row] = lse_of(M, wsum) * kLn2;
   } else {
     if (lane == 0) m_s[w] = M, l_s[w] = wsum;
 #pragma unroll
@@ -1407,10 +1487,10 @@ paged_combine_kernel(PagedAttnParams p) {
       f[u] = m_s[u] == -INFINITY ? 0.f : fast_exp2(m_s[u] - top);
       sum += l_s[u] * f[u];
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     for (int d = threadIdx.x; d < D; d += 256)
       orow[d] = (T)((o_s[0][d] * f[0] + o_s[1][d] * f[1] + o_s[2][d] * f[2] + o_s[3][d] * f[3]) * inv);
-    if (p.lse && threadIdx.x == 0) p.lse[row] = sum > 0.f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
+    if (p.lse && threadIdx.x == 0) p.lse[row] = lse_of(top, sum) * kLn2;
   }
 }
 
@@ -1439,63 +1519,53 @@ paged_merge_kernel(PagedAttnParams p) {
         o += po[s * (D / 4)] * w;
       }
   }
-  o *= sum > 0.f ? 1.f / sum : 0.f;
+  o *= sum == 0.f ? 0.f : 1.f / sum;
   T* orow = (T*)p.o + (c.cu ? t * p.o_ss : b * p.o_sb + n * p.o_ss) + h * p.o_sh;
   *reinterpret_cast<vec4<T>*>(orow + d) = vec4<T>{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
-  if (p.lse && d == 0) p.lse[row] = sum > 0.f ? (M + fast_log2(sum)) * kLn2 : -INFINITY;
+  if (p.lse && d == 0) p.lse[row] = lse_of(M, sum) * kLn2;
 }
 
-#ifndef FAL_PAGED_TILE_OVER
-#define FAL_PAGED_TILE_OVER 1
-#endif
-#ifndef FAL_PAGED_TILE_FROM
-#define FAL_PAGED_TILE_FROM 32
-#endif
-#ifndef FAL_PAGED_WH
-#define FAL_PAGED_WH 4
-#endif
-#ifndef FAL_PAGED_WPC
-#define FAL_PAGED_WPC 1
-#endif
-#ifndef FAL_PAGED_UNIT
-#define FAL_PAGED_UNIT 32
-#endif
-#ifndef FAL_PAGED_DIRECT
-#define FAL_PAGED_DIRECT 2048
-#endif
-PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8, bool packed,
-                     int row_bytes, int ncu) {
+constexpr int kSplitCols = 32;      // most columns of a KV head that the split kernel takes
+constexpr int kDirectRows = 2048;   // longest caches that one workgroup takes whole
+
+PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8,
+                     bool packed, int ncu) {
   PagedPlan r{};
-  r.max_cols = FAL_PAGED_TILE_FROM;
-  const int64_t wide = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
-  if (wide > r.max_cols) {
-    r.row_split = wide <= kTileCols / 2 && d <= 128 ? 2 : 1;
-    const int64_t tile_cols = kTileCols / r.row_split, tiles = (wide + tile_cols - 1) / tile_cols;
+  const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
+  if (cols > kSplitCols) {
+    // The tile kernel.  Splits: as many as fill the workgroup slots (two per compute unit, one at
+    // head dim 256) once, at most 16 and of four tiles at least.
+    r.row_split = cols <= kTileCols / 2 && d <= 128 ? 2 : 1;
+    const int64_t tile_cols = kTileCols / r.row_split, tiles = (cols + tile_cols - 1) / tile_cols;
     r.tile_cols = (int)tiles;
     // column tiles of packed tokens: at most one that is not full in each sequence
-    const int64_t all = std::min(B * tiles, total * (Hq / Hkv) / tile_cols + B);
-    const int64_t blocks = Hkv * all, slots = (int64_t)ncu * (d > 128 ? 1 : 2) * FAL_PAGED_TILE_OVER;
-    const int64_t longest = (capacity + 4 * tile_rows(d) - 1) / (4 * tile_rows(d));   // (four tiles at least)
-    int64_t n = (slots + blocks / 2) / (blocks > 0 ? blocks : 1);
-    n = n > 16 ? 16 : n > longest ? longest : n;
-    r.splits = (int)(n < 1 ? 1 : n);
+    const int64_t all = std::max<int64_t>(std::min(B * tiles, total * (Hq / Hkv) / tile_cols + B), 1);
+    const int64_t blocks = Hkv * all, slots = (int64_t)ncu * (d > 128 ? 1 : 2);
+    const int64_t longest = (capacity + 4 * tile_rows(d) - 1) / (4 * tile_rows(d));
+    const int64_t n = std::min<int64_t>({(slots + blocks / 2) / blocks, 16, longest});
+    r.splits = (int)std::max<int64_t>(n, 1);
     return r;
   }
   const int waves = paged_waves(d, fp8);
-  const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
   r.nc = cols <= 16 || d > 128 ? 1 : 2;   // (head dim 256: two tiles would not fit the registers)
   r.col_tiles = (int)((cols + 16 * r.nc - 1) / (16 * r.nc));
-  r.cols = r.col_tiles * 16 * r.nc;
+  r.cols = (int)cols;
+  // One workgroup per sequence and KV head, and no second kernel, where that is one round of
+  // short ones (1000 rows: 12.9 us, in runs 13.5; 512 workgroups of up to 1500 rows: 41 us, in
+  // runs 36).
+  // (Of one token: results that are not finite under a mask are the second kernel's.)
+  r.direct = capacity <= kDirectRows && !packed && seqlen == 1 && B * Hkv * r.col_tiles <= ncu;
+  // KV heads of a workgroup, by the rows that its run has at most (measured on 32/8 heads of 128,
+  // 8 bits, with 1 / 2 / 4 heads): 4096 x 4 rows 18.7 / 18.5 / 19.8 us, 16 x 8000 43.2 / 41.3 /
+  // 42.6, 64 x 2500 54.5 / 45.5 / 46.6, 32 x 32768 206 / 186 / 178.
   r.wave_heads = 1;
-  r.direct = capacity <= FAL_PAGED_DIRECT && !packed && B * Hkv * r.col_tiles <= ncu;
-  // rows of a run with one, two, four heads to a workgroup: HEADRULE
   const int64_t run_rows = B * capacity * Hkv / ncu;
   if (!r.direct && Hkv % 2 == 0 && run_rows >= 2 * 1280) r.wave_heads = Hkv % 4 == 0 && run_rows >= 4 * 2048 ? 4 : 2;
-  r.unit_rows = FAL_PAGED_UNIT * waves / r.wave_heads;
+  r.unit_rows = 32 * waves / r.wave_heads;   // a step of each wave
+  // one run per compute unit (two: decode of 32 x 32768 rows 178 -> 190 us)
   const int64_t most = B * ((capacity + r.unit_rows - 1) / r.unit_rows + 1);
-  int64_t parts = (int64_t)ncu * FAL_PAGED_WPC / (Hkv / r.wave_heads * r.col_tiles);
-  parts = parts < 1 ? 1 : parts > most ? most : parts;
-  r.parts = (int)(r.direct ? B : parts < 1 ? 1 : parts);
+  const int64_t parts = std::min<int64_t>(ncu / (Hkv / r.wave_heads * r.col_tiles), most);
+  r.parts = (int)(r.direct ? B : std::max<int64_t>(parts, 1));
   return r;
 }
 
@@ -1512,8 +1582,15 @@ static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
     return hipGetLastError();
   }
   const dim3 grid((unsigned)(p.parts * (p.c.Hkv / p.wave_heads) * p.col_tiles)), block(paged_waves(D, FP8) * 64);
-  if (D > 128 || p.nc == 1) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((paged_split_kernel<T, FP8, (D > 128 ? 128 : D), 2>), grid, block, 0, st, p);
+  constexpr int D2 = D > 128 ? 128 : D;   // (two tiles: up to head dim 128)
+  const bool one = p.c.n == 1;
+  if (D > 128 || p.nc == 1) {
+    if (one) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_split_kernel<T, FP8, D, 1, false>), grid, block, 0, st, p);
+  } else {
+    if (one) hipLaunchKernelGGL((paged_split_kernel<T, FP8, D2, 2, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_split_kernel<T, FP8, D2, 2, false>), grid, block, 0, st, p);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.direct) return e;
   const int64_t rows = (int64_t)p.c.total * p.c.Hq;

@@ -319,7 +319,9 @@ int fal_paged_append_bf16(const fal_paged_cache* cache, const void* k, const voi
  * j <= cache_seqlens[b] - n + i (bottom-right alignment); otherwise every token sees all rows.
  *   q, o [tokens, Hq, d]; lse, optional, fp32 [tokens, Hq] contiguous, natural log.  A token that
  *   sees no row, and a row outside every sequence, gets o = 0 and lse = -infinity.
- * workspace: fal_paged_attn_workspace_size bytes (it reads the sizes and fp8 alone).
+ * workspace: fal_paged_attn_workspace_size bytes, for the partial results of runs of rows that
+ * several workgroups share.  The size follows from the sizes, fp8 and whether there are
+ * cu_seqlens, and depends on the current device, as fal_bwd_workspace_best does.
  */
 size_t fal_paged_attn_workspace_size(const fal_paged_cache* cache);
 int fal_paged_attn(const fal_paged_cache* cache, const void* q, void* o, float* lse,

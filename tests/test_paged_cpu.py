@@ -71,6 +71,8 @@ BAD_CACHES = [
     (dict(k_strides=(2 ** 33 + 16, 128, 256)), FAL_ERR_INVALID, "k_cache: stride[0]"),
     (dict(k_scale_strides=(2 ** 31, 1)), FAL_ERR_INVALID, "k_scale: strides must be"),
     (dict(v_strides=(2 ** 30, 128, 2 ** 22)), FAL_ERR_UNSUPPORTED, "v_cache: row stride"),
+    (dict(page_size=1024, max_pages=1, k_strides=(2 ** 32, 128, 2 ** 21 + 16), v_strides=(2 ** 32, 128, 256)), FAL_ERR_UNSUPPORTED,
+     "k_cache: a page of 1024 rows"),
     (dict(v_strides=(16384, 128, 112)), FAL_ERR_UNSUPPORTED, "shorter than a row"),
     (dict(k_scale=None), FAL_ERR_INVALID, "k_scale: null pointer"),
     (dict(v_scale=P + 2), FAL_ERR_INVALID, "v_scale: base pointer must be 4-byte aligned"),
@@ -118,6 +120,16 @@ def test_append_refuses(ext):
     c = cache(ext, total_tokens=0, seqlen=0, k_strides=(2 * 16384, 128, 256), v_strides=(128, 1280, 2560),
               k_scale_strides=(1, 10))
     assert append(ext, c) == (FAL_OK, "")
+
+
+def test_workspace_size(ext):
+    """Nothing for calls that are not recognised, and no more for a hint past the tokens there are."""
+    size = lambda **kw: ext._lib.fal_paged_attn_workspace_size(ctypes.byref(cache(ext, **kw)))
+    assert ext._lib.fal_paged_attn_workspace_size(None) == 0
+    for kw in (dict(heads_q=7), dict(heads_kv=0), dict(page_size=0), dict(max_pages=-1), dict(batch=-1), dict(seqlen=2 ** 40)):
+        assert size(**kw) == 0
+    assert size(batch=64, seqlen=64, total_tokens=64, cu_seqlens=P, max_pages=1000) == \
+        size(batch=64, seqlen=10 ** 9, total_tokens=64, cu_seqlens=P, max_pages=1000)
 
 
 def test_attention_refuses(ext):

@@ -391,6 +391,61 @@ def test_attend_stale_rows_and_missing_pages(cache, n):
 
 
 @pytest.mark.parametrize("cache", ["fp8", "same"])
+@pytest.mark.parametrize("rows", [40, 3000])
+@pytest.mark.parametrize("n", [1, 3, 12, 40])
+def test_attend_not_finite(cache, rows, n):
+    """A NaN key makes the tokens that see it NaN and no others; an infinite value is infinite in the
+    result; the other sequence's rows are as they were."""
+    pool = Pool(2, rows // 16 + 2, 16, 2, 64, cache, torch.bfloat16, seed=20)
+    q = randn((2, n, 8, 64), 1, torch.bfloat16, 0.05)
+    lens = [rows, rows - 3]
+    clean = pool.attend(q, lens, return_softmax_lse=True)
+    at, slot = int(pool.table[0, (rows - 1) // 16]), (rows - 1) % 16
+    pool.rows(pool.k_cache)[at, slot, 0, 7] = math.nan            # the last row, KV head 0
+    o, lse = pool.attend(q, lens, return_softmax_lse=True)
+    assert bool(torch.isnan(o[0, -1, :4]).all()) and bool(torch.isnan(lse[0, -1, :4]).all())
+    for a, b in ((o, clean[0]), (lse, clean[1])):
+        assert torch.equal(a[1], b[1]) and torch.equal(a[0, :, 4:], b[0, :, 4:]) and torch.equal(a[0, :-1], b[0, :-1])
+    pool.rows(pool.k_cache)[at, slot, 0, 7] = 0
+    clean = pool.attend(q, lens, return_softmax_lse=True)
+    # values: the last row, which the last token alone sees, and an early one
+    near = 4 * 2.0 ** -8 * float(pool.rows(pool.v_cache).float().abs().max()) * (1 if cache == "same" else 2.0 ** -4)
+    early = int(pool.table[1, 0])
+    pool.rows(pool.v_cache)[at, slot, 0, 5] = math.nan
+    if cache == "same":
+        pool.rows(pool.v_cache)[early, 2, 1, 5] = math.inf
+    o, lse = pool.attend(q, lens, return_softmax_lse=True)
+    want_nan, want_inf = torch.zeros_like(o, dtype=torch.bool), torch.zeros_like(o, dtype=torch.bool)
+    want_nan[0, -1, :4, 5] = True
+    for i in range(n):
+        want_inf[1, i, 4:, 5] = cache == "same" and lens[1] - n + i >= 2
+    assert torch.equal(torch.isnan(o), want_nan) and torch.equal(o == math.inf, want_inf)
+    rest = ~(want_nan | want_inf)
+    # two results of rounded probabilities: each within 2 u of sum p |v| <= max |v|
+    assert float((o.float() - clean[0].float()).abs()[rest].max()) <= near
+    seen = torch.isfinite(clean[1])
+    assert torch.equal(torch.isfinite(lse), seen) and float((lse - clean[1])[seen].abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("n", [1, 5])
+def test_attend_hundreds_of_sequences(n):
+    """More sequences than are read at once, some of them empty, in runs that hold many of them."""
+    g = torch.Generator().manual_seed(5)
+    lens = [int(x) if int(x) > 20 else 0 for x in torch.randint(0, 130, (700,), generator=g)]
+    lens[3], lens[699] = 2100, 2090
+    pool = Pool(1, 2200, 16, 2, 32, "fp8", seed=21)
+    table = torch.zeros((700, 132), dtype=torch.int32)
+    at = 0
+    for b, m in enumerate(lens):
+        used = -(-m // 16)
+        table[b, :used] = pool.table[0, at:at + used].cpu()
+        at = (at + used) % 2000
+    pool.table = table.cuda()
+    q = randn((700, n, 4, 32), 1)
+    check_attend(pool, q, lens, [n] * 700, pool.attend(q, lens, return_softmax_lse=True))
+
+
+@pytest.mark.parametrize("cache", ["fp8", "same"])
 @pytest.mark.parametrize("n", [1, 24])
 def test_attend_many_sequences(cache, n):
     """More sequences than a wave has lanes, most of them short."""
@@ -407,7 +462,8 @@ def test_attend_many_sequences(cache, n):
 def test_attend_packed_rows_outside_every_sequence(cache):
     pool = Pool(3, 5, 16, 2, 64, cache, seed=11)
     q = randn((60, 4, 64), 1)
-    for first, hint in ((4, 33), (0, 1)):      # (the longest sequence's length is only a hint)
+    # (the longest sequence's length only sizes the grid: 20 is the tile kernel, one column tile of two)
+    for first, hint in ((4, 33), (0, 1), (0, 0), (4, 20), (4, 10 ** 9)):
         cu = torch.tensor([first, 9, 9, 42], dtype=torch.int32).cuda()
         lens = [30, 8, 77]
         o, lse = pool.attend(q, lens, cu_seqlens_q=cu, max_seqlen_q=hint, return_softmax_lse=True)
