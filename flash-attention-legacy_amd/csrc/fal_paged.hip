@@ -396,13 +396,13 @@ hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st
 // A column is one (token, query head) of a KV head: column c of a sequence is token c / G and
 // head c % G of the group of G heads.  The rows of all sequences, in units, are cut into `parts`
 // equal runs (see Runs); one workgroup takes one run for NC tiles of 16 columns and one, two or
-// four KV heads, and its four waves share the heads and then the rows: each takes 32-row steps
-// in turn, as two slices of 16 rows (a slice lies in one page), with no barrier until the merge
+// four KV heads, and its waves share the heads and then the rows: each takes 32-row steps in
+// turn, as two slices of 16 rows (a slice lies in one page), with no barrier until the merge
 // at the end of a sequence or of the run.
 // Equal runs: with fixed chunks of each sequence, 32 sequences of 1k to 32k rows left a tail of
 // half-empty rounds, and grids sized for the page table's capacity were mostly empty.
-// Several heads: rows of 128 bytes, one head's of many, reach 5.0 TB/s, four heads' side by side
-// RATE4 (32 sequences of 16k rows, 8 KV heads).
+// Several heads: rows of 128 bytes, one head's of many, reach 5.3 TB/s, four heads' side by side
+// 6.0 (32 sequences of 16384 rows, 8 KV heads).
 // * S^T = K Q^T on 16x16x32 MFMA, M = 16 rows, N = 16 columns: every K and V byte is read once
 //   for all columns of the tile.
 // * K rows go straight to registers in MFMA order, two steps ahead; e4m3 codes become 16-bit
@@ -412,7 +412,10 @@ hipError_t launch_paged_append(const PagedAppendParams& p, int d, hipStream_t st
 // * A page's key scale multiplies its scores.  Its value scale multiplies P relative to the
 //   largest seen so far, which O is kept in units of, so P stays in [0, 1] and no 16-bit value
 //   leaves its type's range whatever the scales are.
-// Bound by reading the cache.
+// Bound by reading the cache (32 sequences of 1k to 32k rows, 32/8 heads of 128, 8 bits: 177 us,
+// 6.2 TB/s; 16 bits 335 us, 6.6 TB/s); calls of some ten MB by the chain of dependent loads
+// (lengths, page table, rows: 5 to 7 us) at the start and the merge at the end.
+
 // Waves of a workgroup of the split kernel: eight where their rings fit the LDS.
 __host__ __device__ constexpr int paged_waves(int d, bool fp8) { return d <= 128 || fp8 ? 8 : 4; }
 
@@ -708,7 +711,7 @@ paged_split_kernel(PagedAttnParams p) {
   const uint8_t* vread = FP8 ? ring + (kk >> 2) * VS::BYTES + vr * VROW + 8 * (l16 & 1) : ring + vr * VROW + 8 * (l16 & 1);
   const int vc0 = FP8 ? VS::swz(vr, kk >> 2) : ((l16 >> 1) & 1) ^ VS::swz(vr, 0);
 
-  for (; left > 0; ++b, local = 0) {
+  for (; left > 0 && b < c.B; ++b, local = 0) {
     const int L = cache_rows(c, b);
     const int take = min(left, (L > 0 ? cdiv(L, p.unit_rows) + 1 : 0) - local);
     left = p.direct ? 0 : left - take;
@@ -750,158 +753,158 @@ paged_split_kernel(PagedAttnParams p) {
     // wr + NR * (i / 2).  Byte offsets of its first rows, the rows it has (0: none, or a page
     // outside the pool) and its scales.
     for (int k_begin = row0; k_begin < row1; k_begin += 1024 * NR) {
-    const int k_end = min(row1, k_begin + 1024 * NR);
-    const int nsteps = cdiv(k_end - k_begin, 32);
-    int64_t koff = 0, voff = 0;
-    int nrow = 0;
-    float ksc = 1.f, vsc = 1.f;
-    {
-      const int r = k_begin + (wr + NR * (lane >> 1)) * 32 + (lane & 1) * 16;
-      if (r < k_end) {
-        const int page = r / c.page_size, slot = r - page * c.page_size;
-        const int pid = c.table[b * c.table_sb + page];
-        if (pid >= 0 && pid < c.num_pages) {
-          nrow = min(16, k_end - r);
-          koff = ((uint64_t)(uint32_t)pid * k_page << 4) + (uint32_t)(slot * k_ss);
-          voff = ((uint64_t)(uint32_t)pid * v_page << 4) + (uint32_t)(slot * v_ss);
-          if (FP8) {
-            ksc = kscale[(uint64_t)(uint32_t)pid * (uint32_t)c.ks_sp];
-            vsc = vscale[(uint64_t)(uint32_t)pid * (uint32_t)c.vs_sp];
+      const int k_end = min(row1, k_begin + 1024 * NR);
+      const int nsteps = cdiv(k_end - k_begin, 32);
+      int64_t koff = 0, voff = 0;
+      int nrow = 0;
+      float ksc = 1.f, vsc = 1.f;
+      {
+        const int r = k_begin + (wr + NR * (lane >> 1)) * 32 + (lane & 1) * 16;
+        if (r < k_end) {
+          const int page = r / c.page_size, slot = r - page * c.page_size;
+          const int pid = c.table[b * c.table_sb + page];
+          if (pid >= 0 && pid < c.num_pages) {
+            nrow = min(16, k_end - r);
+            koff = ((uint64_t)(uint32_t)pid * k_page << 4) + (uint32_t)(slot * k_ss);
+            voff = ((uint64_t)(uint32_t)pid * v_page << 4) + (uint32_t)(slot * v_ss);
+            if (FP8) {
+              ksc = kscale[(uint64_t)(uint32_t)pid * (uint32_t)c.ks_sp];
+              vsc = vscale[(uint64_t)(uint32_t)pid * (uint32_t)c.vs_sp];
+            }
           }
         }
       }
-    }
-    auto issue = [&](int jj, int buf) {   // the wave's step jj
-  #pragma unroll
-      for (int sl = 0; sl < 2; ++sl) {
-        const int i = 2 * jj + sl;
-        const int n = (int)lane_of((uint32_t)nrow, i);
-        const int64_t ko = (int64_t)(((uint64_t)lane_of((uint32_t)(koff >> 32), i) << 32) | lane_of((uint32_t)koff, i));
-        const int64_t vo = (int64_t)(((uint64_t)lane_of((uint32_t)(voff >> 32), i) << 32) | lane_of((uint32_t)voff, i));
-        const auto krs = make_rsrc(kbase + ko, n > 0 ? (uint32_t)((n - 1) * k_ss + D * CB) : 0);
-        const auto vrs = make_rsrc(vbase + vo, n > 0 ? (uint32_t)((n - 1) * v_ss + D * CB) : 0);
-  #pragma unroll
-        for (int t = 0; t < KL; ++t) {
-          const bool pair = LINE && (t | 1) < KL;
-          // whole lines are read once and evicted first; halves stay until the other half is read
-          kreg[buf][sl][t] = pair ? __builtin_amdgcn_raw_buffer_load_b128(krs, kvl + (t & 1) * 8 * k_ss + (t & ~1) * 64, 0, 2)
-                                  : __builtin_amdgcn_raw_buffer_load_b128(krs, kv0 + t * 64, 0, 0);
-        }
-        if constexpr (KTAIL)
-          ktail[buf][sl] = __builtin_amdgcn_raw_buffer_load_b64(krs, l16 * k_ss + KL * 64 + g4 * 8, 0, 0);
-  #pragma unroll
-        for (int I = 0; I < VS::LOADS; ++I)
-          buffer_to_lds16<2>(vrs, vv[sl][I], ring + (buf * 2 + sl) * VS::BYTES + I * 1024);
-      }
-    };
-    int j = wr;          // this wave's steps: wr, wr + NR, ...
-    if (j < nsteps) issue(0, 0);
-    if (j + NR < nsteps) issue(1, 1);
-    auto step = [&](auto bufc, int jj) {
-      constexpr int buf = decltype(bufc)::value;
-      if (j + NR < nsteps) wait_vmcnt_n<LPS>();
-      else wait_vmcnt_n<0>();
-      f32x4 s[NC][2];
-      float vfac[2], back = 1.f;
+      auto issue = [&](int jj, int buf) {   // the wave's step jj
 #pragma unroll
-      for (int sl = 0; sl < 2; ++sl) {
-        V8 kop[KS];
-        if constexpr (LINE) {
-#pragma unroll
-          for (int t = 0; t + 1 < KL; t += 2) unswap_lines(kreg[buf][sl][t], kreg[buf][sl][t + 1]);
-        }
-        if constexpr (FP8) {
+        for (int sl = 0; sl < 2; ++sl) {
+          const int i = 2 * jj + sl;
+          const int n = (int)lane_of((uint32_t)nrow, i);
+          const int64_t ko = (int64_t)(((uint64_t)lane_of((uint32_t)(koff >> 32), i) << 32) | lane_of((uint32_t)koff, i));
+          const int64_t vo = (int64_t)(((uint64_t)lane_of((uint32_t)(voff >> 32), i) << 32) | lane_of((uint32_t)voff, i));
+          const auto krs = make_rsrc(kbase + ko, n > 0 ? (uint32_t)((n - 1) * k_ss + D * CB) : 0);
+          const auto vrs = make_rsrc(vbase + vo, n > 0 ? (uint32_t)((n - 1) * v_ss + D * CB) : 0);
 #pragma unroll
           for (int t = 0; t < KL; ++t) {
-            kop[2 * t] = e4m3_to_16<T>(kreg[buf][sl][t][0], kreg[buf][sl][t][1]);
-            kop[2 * t + 1] = e4m3_to_16<T>(kreg[buf][sl][t][2], kreg[buf][sl][t][3]);
+            const bool pair = LINE && (t | 1) < KL;
+            // whole lines are read once and evicted first; halves stay until the other half is read
+            kreg[buf][sl][t] = pair ? __builtin_amdgcn_raw_buffer_load_b128(krs, kvl + (t & 1) * 8 * k_ss + (t & ~1) * 64, 0, 2)
+                                    : __builtin_amdgcn_raw_buffer_load_b128(krs, kv0 + t * 64, 0, 0);
           }
-          if constexpr (KTAIL) kop[KS - 1] = e4m3_to_16<T>(ktail[buf][sl][0], ktail[buf][sl][1]);
-        } else {
+          if constexpr (KTAIL)
+            ktail[buf][sl] = __builtin_amdgcn_raw_buffer_load_b64(krs, l16 * k_ss + KL * 64 + g4 * 8, 0, 0);
 #pragma unroll
-          for (int t = 0; t < KS; ++t) kop[t] = __builtin_bit_cast(V8, kreg[buf][sl][t]);
+          for (int I = 0; I < VS::LOADS; ++I)
+            buffer_to_lds16<2>(vrs, vv[sl][I], ring + (buf * 2 + sl) * VS::BYTES + I * 1024);
         }
+      };
+      int j = wr;          // this wave's steps: wr, wr + NR, ...
+      if (j < nsteps) issue(0, 0);
+      if (j + NR < nsteps) issue(1, 1);
+      auto step = [&](auto bufc, int jj) {
+        constexpr int buf = decltype(bufc)::value;
+        if (j + NR < nsteps) wait_vmcnt_n<LPS>();
+        else wait_vmcnt_n<0>();
+        f32x4 s[NC][2];
+        float vfac[2], back = 1.f;
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl) {
+          V8 kop[KS];
+          if constexpr (LINE) {
+#pragma unroll
+            for (int t = 0; t + 1 < KL; t += 2) unswap_lines(kreg[buf][sl][t], kreg[buf][sl][t + 1]);
+          }
+          if constexpr (FP8) {
+#pragma unroll
+            for (int t = 0; t < KL; ++t) {
+              kop[2 * t] = e4m3_to_16<T>(kreg[buf][sl][t][0], kreg[buf][sl][t][1]);
+              kop[2 * t + 1] = e4m3_to_16<T>(kreg[buf][sl][t][2], kreg[buf][sl][t][3]);
+            }
+            if constexpr (KTAIL) kop[KS - 1] = e4m3_to_16<T>(ktail[buf][sl][0], ktail[buf][sl][1]);
+          } else {
+#pragma unroll
+            for (int t = 0; t < KS; ++t) kop[t] = __builtin_bit_cast(V8, kreg[buf][sl][t]);
+          }
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc) {
+            s[nc][sl] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < KS; ++t) s[nc][sl] = mfma16(kop[t], qreg[nc][t], s[nc][sl]);
+          }
+        }
+        const int n0 = (int)lane_of((uint32_t)nrow, 2 * jj), n1 = (int)lane_of((uint32_t)nrow, 2 * jj + 1);
+        // scores stay unscaled until their exponent: max and mask commute with a positive factor
+        float kfac[2] = {p.scale_log2, p.scale_log2};
+        if constexpr (FP8) {
+          kfac[0] = fmaxf(kfac[0] * lane_of(ksc, 2 * jj), 0x1p-126f), kfac[1] = fmaxf(kfac[1] * lane_of(ksc, 2 * jj + 1), 0x1p-126f);
+          const float v0 = n0 > 0 ? lane_of(vsc, 2 * jj) : 0.f, v1 = n1 > 0 ? lane_of(vsc, 2 * jj + 1) : 0.f;
+          const float now = fmaxf(ref, fmaxf(v0, v1));
+          const float inv = now >= 0x1p-126f ? __builtin_amdgcn_rcpf(now) : 0.f;
+          vfac[0] = v0 * inv, vfac[1] = v1 * inv, back = ref * inv;
+          ref = now;
+        }
+        const int r0 = k_begin + j * 32;
+        const bool whole = n0 == 16 && n1 == 16 && (ONE || r0 + 32 <= lim_first);   // every row seen by every column
+        V8 pb[NC];
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-          s[nc][sl] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (!whole) {
 #pragma unroll
-          for (int t = 0; t < KS; ++t) s[nc][sl] = mfma16(kop[t], qreg[nc][t], s[nc][sl]);
-        }
-      }
-      const int n0 = (int)lane_of((uint32_t)nrow, 2 * jj), n1 = (int)lane_of((uint32_t)nrow, 2 * jj + 1);
-      // scores stay unscaled until their exponent: max and mask commute with a positive factor
-      float kfac[2] = {p.scale_log2, p.scale_log2};
-      if constexpr (FP8) {
-        kfac[0] = fmaxf(kfac[0] * lane_of(ksc, 2 * jj), 0x1p-126f), kfac[1] = fmaxf(kfac[1] * lane_of(ksc, 2 * jj + 1), 0x1p-126f);
-        const float v0 = n0 > 0 ? lane_of(vsc, 2 * jj) : 0.f, v1 = n1 > 0 ? lane_of(vsc, 2 * jj + 1) : 0.f;
-        const float now = fmaxf(ref, fmaxf(v0, v1));
-        const float inv = now >= 0x1p-126f ? __builtin_amdgcn_rcpf(now) : 0.f;
-        vfac[0] = v0 * inv, vfac[1] = v1 * inv, back = ref * inv;
-        ref = now;
-      }
-      const int r0 = k_begin + j * 32;
-      const bool whole = n0 == 16 && n1 == 16 && (ONE || r0 + 32 <= lim_first);   // every row seen by every column
-      V8 pb[NC];
+            for (int sl = 0; sl < 2; ++sl)
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) {
-        if (!whole) {
+              for (int i = 0; i < 4; ++i) {
+                const int r = 4 * g4 + i;
+                if (r >= (sl ? n1 : n0) || (!ONE && r0 + sl * 16 + r >= lim[nc])) s[nc][sl][i] = -INFINITY;
+              }
+          }
+          float mx = fmaxf(fmaxf(fmaxf(s[nc][0][0], s[nc][0][1]), fmaxf(s[nc][0][2], s[nc][0][3])) * kfac[0],
+                           fmaxf(fmaxf(s[nc][1][0], s[nc][1][1]), fmaxf(s[nc][1][2], s[nc][1][3])) * kfac[1]);
+          mx = quarters_max(mx);
+          const float m_new = fmaxf(m_run[nc], mx);
+          const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
+          float l = 0.f;
 #pragma unroll
           for (int sl = 0; sl < 2; ++sl)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int r = 4 * g4 + i;
-              if (r >= (sl ? n1 : n0) || (!ONE && r0 + sl * 16 + r >= lim[nc])) s[nc][sl][i] = -INFINITY;
+              const float e = fast_exp2(fmaf(s[nc][sl][i], kfac[sl], -m_use));
+              l += e;
+              pb[nc][sl * 4 + i] = (T)(FP8 ? e * vfac[sl] : e);
             }
-        }
-        float mx = fmaxf(fmaxf(fmaxf(s[nc][0][0], s[nc][0][1]), fmaxf(s[nc][0][2], s[nc][0][3])) * kfac[0],
-                         fmaxf(fmaxf(s[nc][1][0], s[nc][1][1]), fmaxf(s[nc][1][2], s[nc][1][3])) * kfac[1]);
-        mx = quarters_max(mx);
-        const float m_new = fmaxf(m_run[nc], mx);
-        const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
-        float l = 0.f;
+          if (__any(m_new != m_run[nc]) || (FP8 && back != 1.f)) {
+            const float alpha = fast_exp2(m_run[nc] - m_use);
+            l_run[nc] *= alpha;
+            m_run[nc] = m_new;
+            const float f = FP8 ? alpha * back : alpha;
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = fast_exp2(fmaf(s[nc][sl][i], kfac[sl], -m_use));
-            l += e;
-            pb[nc][sl * 4 + i] = (T)(FP8 ? e * vfac[sl] : e);
+            for (int db = 0; db < DBN; ++db) oacc[nc][db] *= f;
           }
-        if (__any(m_new != m_run[nc]) || (FP8 && back != 1.f)) {
-          const float alpha = fast_exp2(m_run[nc] - m_use);
-          l_run[nc] *= alpha;
-          m_run[nc] = m_new;
-          const float f = FP8 ? alpha * back : alpha;
-#pragma unroll
-          for (int db = 0; db < DBN; ++db) oacc[nc][db] *= f;
+          l_run[nc] += l;
         }
-        l_run[nc] += l;
-      }
-      // O^T += V^T P^T over the 32 rows
+        // O^T += V^T P^T over the 32 rows
 #pragma unroll
-      for (int db = 0; db < DBN; ++db) {
-        V8 vop;
-        if constexpr (FP8) {
-          const u32x2 x = lds_tr8(vread + buf * 2 * VS::BYTES + ((db ^ vc0) << 4));
-          vop = e4m3_to_16<T>(x[0], x[1]);
-        } else {
-          const T* v0 = (const T*)(vread + buf * 2 * VS::BYTES + ((vc0 ^ (2 * db)) << 4));
-          vop = join8(lds_tr(v0), lds_tr((const T*)((const uint8_t*)v0 + VS::BYTES)));
+        for (int db = 0; db < DBN; ++db) {
+          V8 vop;
+          if constexpr (FP8) {
+            const u32x2 x = lds_tr8(vread + buf * 2 * VS::BYTES + ((db ^ vc0) << 4));
+            vop = e4m3_to_16<T>(x[0], x[1]);
+          } else {
+            const T* v0 = (const T*)(vread + buf * 2 * VS::BYTES + ((vc0 ^ (2 * db)) << 4));
+            vop = join8(lds_tr(v0), lds_tr((const T*)((const uint8_t*)v0 + VS::BYTES)));
+          }
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc) oacc[nc][db] = mfma16(vop, pb[nc], oacc[nc][db]);
         }
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc) oacc[nc][db] = mfma16(vop, pb[nc], oacc[nc][db]);
+        // LDS reads of this buffer must finish before the next copies overwrite it
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (j + 2 * NR < nsteps) issue(jj + 2, buf);
+        j += NR;
+      };
+      // two steps per trip so that the ring index is a compile-time constant
+      for (int jj = 0; j < nsteps; jj += 2) {
+        step(std::integral_constant<int, 0>{}, jj);
+        if (j >= nsteps) break;
+        step(std::integral_constant<int, 1>{}, jj + 1);
       }
-      // LDS reads of this buffer must finish before the next copies overwrite it
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (j + 2 * NR < nsteps) issue(jj + 2, buf);
-      j += NR;
-    };
-    // two steps per trip so that the ring index is a compile-time constant
-    for (int jj = 0; j < nsteps; jj += 2) {
-      step(std::integral_constant<int, 0>{}, jj);
-      if (j >= nsteps) break;
-      step(std::integral_constant<int, 1>{}, jj + 1);
-    }
     }
 
     // ---- the piece's partial output, normalised, and its log2-domain LSE; or the result ----
@@ -981,15 +984,19 @@ paged_split_kernel(PagedAttnParams p) {
 // two waves share a column's rows: half of the matrix units would idle otherwise), and
 // walks tiles of 64 or 32 rows; with few workgroups, `splits` of them share a column tile's rows.
 // * Each wave brings a slice of the tile (16 rows of one page, or half of one) from the cache: its
-//   page and scales are scalars, its lanes' places in the page constants, and e4m3 codes become 16-bit values
-//   once, on the way to LDS, not once per wave that reads them.  Loads of a tile run a whole
-//   tile ahead, its page number two.
+//   page and scales are scalars, its lanes' places in the page constants, and e4m3 codes become
+//   16-bit values once, on the way to LDS, not once per wave that reads them.  Loads of a tile
+//   run a whole tile ahead, its page number two.
 // * S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMA; the S^T accumulators are P^T's operand in
 //   place (fal_common.h).
 // * The running maximum that exponents are taken from moves only when a score passes it by 8:
 //   P reaches 2^8 at most, and the accumulators are rarely rescaled.
 // * Scales as in the split kernel: the value factor enters the exponent, and each slice's sum is
 //   divided by it again for l.
+// * Each group of LDS reads goes out before the products of the group before it (chunk of 1024
+//   tokens behind 8192 rows, 32/8 heads of 128, 8 bits: 234 -> 184 us).
+// Bound by the vector units (ten instructions per matrix instruction, 32 % of the matrix units'
+// time used at 234 us): that chunk runs at 790 TFLOP/s, in 16 bits at 860.
 constexpr int kTileCols = 128;
 // Tiles in LDS: swizzled rows, or for head dim 96 rows padded to 208 bytes, of which any sixteen
 // start on different 16-byte pieces of the 256 that the banks hold.
@@ -1015,7 +1022,7 @@ __device__ __forceinline__ const P& args_again() {
 
 // Column `col` of sequence b and KV head hkv over the rows r0 .. r1 of a split, by one wave (see
 // attend_alone).  Not inlined: it is hardly ever reached, and inlined it took registers from the
-// loop (chunk of 1024 tokens behind 8192 rows: ALONE0).
+// loop (chunk of 1024 tokens behind 8192 rows 185 -> 193 us).
 template <class T, bool FP8, int D>
 __device__ __attribute__((noinline)) void column_again(const PagedAttnParams& p, int b, int hkv, int col, int split, int r0, int r1) {
   const PagedCache& c = p.c;
@@ -1380,7 +1387,7 @@ paged_tile_kernel(PagedAttnParams p) {
 // Merge the pieces' partial outputs of (token, query head) rows, W waves to a row and four waves
 // to a workgroup.  Each wave takes every W-th piece, eight of them in flight, with weights
 // relative to its own largest LSE; four waves of a row meet in LDS in a fixed order.  (One wave
-// for rows of few pieces: 10240 rows of about four, 34 -> COMB1 us.)
+// for rows of few pieces: 10240 rows of about four, 34 -> 13 us.)
 template <class T, bool FP8, int D, int W>
 __global__ void __launch_bounds__(256)
 paged_combine_kernel(PagedAttnParams p) {
