@@ -895,6 +895,8 @@ int fill_paged(PagedCache& p, const fal_paged_cache* cache, int bf16, bool writt
       (rc = check_scale("k_scale", c, c.k_scale, c.k_scale_strides, written)) ||
       (rc = check_scale("v_scale", c, c.v_scale, c.v_scale_strides, written)))
     return rc;
+  if (written && c.num_pages > 0 && (c.k == c.v || (c.fp8 && c.k_scale == c.v_scale)))
+    return fail(FAL_ERR_INVALID, "keys and values must not share a cache or scales");
   p.k = c.k, p.v = c.v, p.k_scale = c.k_scale, p.v_scale = c.v_scale;
   p.table = c.page_table, p.table_sb = c.table_stride;
   p.seqlens = c.cache_seqlens, p.cu = c.cu_seqlens;

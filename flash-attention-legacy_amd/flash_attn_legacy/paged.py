@@ -71,7 +71,8 @@ def paged_kvcache_append(
     Token i of sequence b becomes row ``cache_seqlens[b] + i``, that is row
     ``(cache_seqlens[b] + i) % page_size`` of page ``page_table[b, (cache_seqlens[b] + i) // page_size]``.
     Rows past the page table's last page and rows of pages outside the pool are dropped.  A page
-    that is written must belong to one sequence only.
+    that is written must belong to one sequence only, and keys and values have a cache and scales
+    each (they may be views of one pool).
 
     Caches of k's type hold the rows rounded once.  float8_e4m3fn caches hold codes, and
     ``code * scale[page, head]`` is the value.  The scale of a page that the call writes becomes

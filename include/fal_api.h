@@ -267,7 +267,7 @@ int fal_decode_noalloc(const void* q, const void* k_cache, const void* v_cache,
  */
 typedef struct fal_paged_cache {
   void* k;                        /* 16-byte aligned */
-  void* v;
+  void* v;                        /* for the append another pointer than k, as v_scale than k_scale */
   float* k_scale;                 /* fp32, entry (page, head) at page * strides[0] + head * strides[1] */
   float* v_scale;
   const int32_t* page_table;      /* device int32 [batch, max_pages], rows table_stride apart */

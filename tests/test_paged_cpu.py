@@ -9,6 +9,7 @@ import torch
 
 FAL_OK, FAL_ERR_INVALID, FAL_ERR_UNSUPPORTED, FAL_ERR_LAUNCH, FAL_ERR_WORKSPACE = range(5)
 P = 4096     # an aligned address that no call gets as far as using
+V = P + (1 << 40)     # the values' cache and scales
 
 
 def s3(*v):
@@ -17,7 +18,7 @@ def s3(*v):
 
 def cache(ext, **kw):
     page, hkv, d = kw.get("page_size", 64), kw.get("heads_kv", 2), kw.get("head_dim", 128)
-    c = ext.PagedCache(k=P, v=P, k_scale=P, v_scale=P, page_table=P, cache_seqlens=P, table_stride=4, batch=3,
+    c = ext.PagedCache(k=P, v=V, k_scale=P, v_scale=V, page_table=P, cache_seqlens=P, table_stride=4, batch=3,
                        seqlen=1, total_tokens=3, heads_q=8, heads_kv=2, head_dim=128, num_pages=10, page_size=64,
                        max_pages=4, fp8=1)
     c.k_strides[:] = c.v_strides[:] = (page * hkv * d, d, hkv * d)
@@ -102,6 +103,8 @@ def test_append_refuses(ext):
             (dict(), dict(k_scale_strides=(0, 1)), "k_scale: entries overlap"),
             (dict(), dict(v_scale_strides=(1, 1)), "v_scale: entries overlap"),
             (dict(), dict(v_scale_strides=(1, 9)), "v_scale: entries overlap"),
+            (dict(), dict(v=P), "must not share a cache or scales"),
+            (dict(), dict(v_scale=P), "must not share a cache or scales"),
             (dict(k=None), {}, "k: null pointer"),
             (dict(k=P + 2), {}, "k: base pointer must be 16-byte aligned"),
             (dict(q_out=None), {}, "q_out: null pointer"),

@@ -638,6 +638,51 @@ def test_other_streams_and_repeats():
     assert all(torch.equal(o, want) for o in outs)
 
 
+# ---- ways of use -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cache", ["fp8", "same"])
+def test_prompt_and_single_tokens_in_one_batch(cache):
+    """A scheduler's step: one prompt's chunk packed with the tokens of running sequences and an
+    empty one; the append and the attention behind it."""
+    lens, new = [100, 37, 500, 0, 64, 15, 333, 1, 250], [1, 1, 300, 0, 1, 1, 1, 1, 1]
+    pool = Pool(len(lens), 26, 32, 2, 128, cache, torch.bfloat16, seed=31)
+    total, cu = sum(new), torch.tensor(starts_of(new), dtype=torch.int32).cuda()
+    k, v, q = (randn((total, h, 128), i, torch.bfloat16) for i, h in enumerate((2, 2, 8)))
+    before = snapshot(pool)
+    assert torch.equal(pool.append(k, v, lens, q=q, cu_seqlens=cu, max_seqlen=300), q)
+    check_append(pool, k, v, lens, new, before)
+    after = [a + n for a, n in zip(lens, new)]
+    got = pool.attend(q, after, return_softmax_lse=True, cu_seqlens_q=cu, max_seqlen_q=300)
+    check_attend(pool, q, after, new, got)
+
+
+@pytest.mark.parametrize("cache", ["fp8", "same"])
+def test_rejected_tokens_are_written_over(cache):
+    """Speculative decoding: five tokens proposed, two kept, the next five start behind those."""
+    pool = Pool(2, 3, 32, 2, 64, cache, seed=17)
+    for step, lens in enumerate(([20, 30], [22, 32], [24, 33])):
+        k, v = randn((10, 2, 64), 2 * step, scale=3.0 ** step), randn((10, 2, 64), 2 * step + 1, scale=9.0 - 4 * step)
+        before = snapshot(pool)
+        pool.append(k.view(2, 5, 2, 64), v.view(2, 5, 2, 64), lens)
+        check_append(pool, k, v, lens, [5, 5], before)
+        q = randn((2, 5, 4, 64), 50 + step)
+        after = [n + 5 for n in lens]
+        check_attend(pool, q, after, [5, 5], pool.attend(q, after, return_softmax_lse=True))
+
+
+@pytest.mark.parametrize("n", [1, 9, 40])
+def test_attend_shared_pages(n):
+    """Sequences with one prefix read the same pages, keys and values may be one cache, and one
+    page may stand in a table twice."""
+    pool = Pool(3, 6, 32, 1, 64, "fp8", seed=5)
+    pool.table[1:, :4] = pool.table[0, :4]
+    pool.table[2, 4] = pool.table[2, 1]
+    pool.v_cache, pool.v_scale = pool.k_cache, pool.k_scale
+    q = randn((3, n, 4, 64), 3)
+    lens = [190, 128 + n, 150]
+    check_attend(pool, q, lens, [n] * 3, pool.attend(q, lens, return_softmax_lse=True))
+
+
 # ---- refusals --------------------------------------------------------------------------------
 
 def test_refusals():
@@ -683,6 +728,8 @@ def test_refusals():
     refused("multiple of 16", append, k, k, kc, vc, table, 1, ks, vs, rotary_cos=cos[:, :4], rotary_sin=cos[:, :4])
     wide = torch.ones((32, 40), device="cuda")
     refused("up to head_dim", append, k, k, kc, vc, table, 1, ks, vs, rotary_cos=wide, rotary_sin=wide)
+    refused("must not share", append, k, k, kc, kc, table, 1, ks, vs)
+    refused("must not share", append, k, k, kc, vc, table, 1, ks, ks)
     refused("rows overlap", append, k, k, kc[:1].expand(7, -1, -1, -1), vc, table, 1, ks, vs)
     refused("entries overlap", append, k, k, kc, vc, table, 1, ks[:1].expand(7, -1), vs)
     refused("divisible", attend, randn((2, 1, 3, 64), 1), kc, vc, table, 1, ks, vs)
