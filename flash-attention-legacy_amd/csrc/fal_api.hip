@@ -960,9 +960,13 @@ int paged_append_impl(const fal_paged_cache* cache, const void* k, const void* v
   p.rotary = (int)rotary_dim, p.interleaved = rotary_interleaved != 0;
   // pages that seqlen rows can touch
   p.pages_per_seq = (int)((std::max<int64_t>(p.c.n, 1) + c.page_size - 2) / c.page_size + 1);
-  if (c.batch * p.pages_per_seq > 0x7fffffff / (2 * c.heads_kv) ||
-      c.batch * p.pages_per_seq * 2 * c.heads_kv + c.total_tokens * c.heads_q * c.head_dim / 16 / 64 >= 0x7fffffff)
+  // of packed sequences each touches at most two pages that its tokens do not fill
+  const int64_t items = batched ? c.batch * p.pages_per_seq
+                                : std::min(c.batch * p.pages_per_seq, c.total_tokens / c.page_size + 2 * c.batch);
+  if (items > 0x7fffffff / (2 * c.heads_kv) ||
+      items * 2 * c.heads_kv + c.total_tokens * c.heads_q * c.head_dim / 16 / 64 >= 0x7fffffff)
     return fail(FAL_ERR_INVALID, "problem too large for one launch");
+  p.page_items = (int)items;
   return launch_status(launch_paged_append(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_append");
 }
 
@@ -999,16 +1003,16 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   const PagedPlan plan = plan_of(c);
   p.parts = plan.parts, p.unit_rows = plan.unit_rows, p.wave_heads = plan.wave_heads;
   p.nc = plan.nc, p.col_tiles = plan.col_tiles, p.cols = plan.cols, p.direct = plan.direct;
-  p.splits = plan.splits, p.tile_cols = plan.tile_cols, p.row_split = plan.row_split;
+  p.splits = plan.splits, p.tile_cols = plan.tile_cols, p.row_split = plan.row_split, p.items = plan.items;
   const size_t rows = paged_partials(plan, c);
   p.part_o = static_cast<float*>(workspace);
   p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(rows * c.head_dim * sizeof(float)));
-  if (c.total_tokens * c.heads_q > 0x7fffffff)
+  if (c.total_tokens * c.heads_q > 0x7ffff000)   // (kernels round columns up to tiles in 32 bits)
     return fail(FAL_ERR_INVALID, "problem too large for one launch");
   if (plan.splits) {
-    const int64_t per = (int64_t)plan.splits * c.heads_kv * plan.tile_cols;
-    if (c.batch > (0x7fffffff - 64) / per) return fail(FAL_ERR_INVALID, "problem too large for one launch");
-    p.tile_blocks = (int)(c.batch * per);
+    const int64_t per = (int64_t)plan.splits * c.heads_kv;
+    if (plan.items > (0x7fffffff - 64) / per) return fail(FAL_ERR_INVALID, "problem too large for one launch");
+    p.tile_blocks = (int)(plan.items * per);
     p.rest_blocks = c.cu_seqlens ? 16 : 0;
   } else if ((int64_t)plan.parts * c.heads_kv * plan.col_tiles > 0x7fffffff ||
              c.batch * ((c.max_pages * c.page_size + plan.unit_rows - 1) / plan.unit_rows + 1) / plan.parts >= 0x7fffffff)

@@ -171,7 +171,8 @@ struct PagedAppendParams {
   int64_t k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, q_sb, q_sh, q_ss, qo_sb, qo_sh, qo_ss;
   int64_t cos_ss, sin_ss;
   int rotary, interleaved;
-  int pages_per_seq;  // 8-bit store blocks per sequence (each walks the touched pages this far apart)
+  int pages_per_seq;  // pages that a sequence's tokens touch at most (all of them of one length)
+  int page_items;     // pages that all tokens touch: 8-bit store blocks per head
   int row_groups;     // groups of heads of a token that are stored row by row
 };
 
@@ -189,8 +190,10 @@ struct PagedAttnParams {
   // per (run, wave_heads KV heads, nc tiles of 16 columns); direct: a run is a sequence, and there
   // is nothing to merge
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
-  // tile kernel (splits > 0): tile_cols column tiles of the longest sequence, each sequence's rows
-  // in `splits` shares; tile_blocks workgroups, and rest_blocks for packed rows outside every sequence
+  // tile kernel (splits > 0): tile_cols column tiles of the longest sequence, `items` of all, each
+  // sequence's rows in `splits` shares; tile_blocks workgroups, and rest_blocks for packed rows
+  // outside every sequence
+  int64_t items;
   int splits, tile_cols, row_split, tile_blocks, rest_blocks;   // row_split: waves that share a column's rows
   float* part_o;      // [parts + B, Hkv, cols, d], or [total, Hq, splits, d]
   float* part_m;      // the same without d: log2-domain LSE
@@ -198,6 +201,7 @@ struct PagedAttnParams {
 struct PagedPlan {
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
   int splits, tile_cols, row_split;
+  int64_t items;
 };
 
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);

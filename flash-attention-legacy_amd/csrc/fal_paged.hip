@@ -43,6 +43,32 @@ __device__ __forceinline__ bool token_place(const PagedCache& c, int t, int& b, 
   return i >= 0 && i < len;
 }
 
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
+
+// Inclusive sum over the wave's lanes (row shifts, then the rows' last lanes broadcast)
+__device__ __forceinline__ int lanes_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31
+  return x;
+}
+
+// Batches are searched by blocks of 64 sequences, one per lane, four blocks read at once: large
+// batches cost one round trip to memory in 256 sequences.
+constexpr int kBlocks = 4;
+
+// Which of `cnt`'s lanes' items, in the lanes' order, the r-th is: the lane; r becomes its place
+// among that lane's.  `sum`: lanes_scan(cnt).
+__device__ __forceinline__ int lane_of_item(uint32_t cnt, uint32_t sum, uint32_t& r) {
+  const auto past = __ballot(sum > r);
+  const int at = past ? __builtin_ctzll(past) : 0;
+  r -= lane_of(sum, at) - lane_of(cnt, at);
+  return at;
+}
+
 // ---------------------------------------------------------------------------
 // Append
 // ---------------------------------------------------------------------------
@@ -213,7 +239,7 @@ __device__ void append_rows(const PagedAppendParams& p, int64_t item) {
 constexpr int kAppendHold = 2, kAppendThreads = 512;
 
 template <int MODE, class T, int D>
-__device__ void append_codes(const PagedAppendParams& p, int b, int h, int first_page, const T* src, int64_t src_ss,
+__device__ void append_codes(const PagedAppendParams& p, int b, int h, int nth, const T* src, int64_t src_ss,
                              uint8_t* cache, int64_t dst_sp, int64_t dst_ss, float* scales, int64_t scale_sp, float* wave_max) {
   constexpr int UPR = D / 16;   // units per row
   const PagedCache& c = p.c;
@@ -223,109 +249,145 @@ __device__ void append_codes(const PagedAppendParams& p, int b, int h, int first
   const int L = max(c.seqlens[b], 0);
   const int64_t end = min((int64_t)L + len, (int64_t)c.capacity);   // rows after the append
   if (c.cu) src += off * src_ss;
-  for (int64_t page = L / c.page_size + first_page; page * c.page_size < end; page += p.pages_per_seq) {
-    const int pid = c.table[b * c.table_sb + page];
-    if (pid < 0 || pid >= c.num_pages) continue;
-    const int64_t first = page * c.page_size;
-    const int r0 = (int)(max((int64_t)L, first) - first);                // first new row of the page
-    const int rows = (int)(min(end, first + c.page_size) - first) - r0;
-    if (rows <= 0) continue;
-    const int64_t i0 = first + r0 - L;                                   // its token
-    const int total = rows * UPR;
-    uint8_t* base = cache + pid * dst_sp;
-    float* sp = scales + pid * scale_sp;
-    const float old = r0 > 0 ? *sp : 0.f;   // filled from its first row on: the old scale is another sequence's
-    auto load = [&](int e, float (&y)[16]) {
-      const int r = e / UPR, u = e % UPR;
-      int ca, cb;
-      unit_chunks<MODE>(u, p.rotary, ca, cb);
-      const T* row = src + (i0 + r) * src_ss;
-      const int64_t pos = first + r0 + r;
-      const vec8<T> a = ld8(row + ca * 8), b8 = ld8(row + cb * 8);
-      const Angles t = unit_angles<MODE>(u, p.rotary, p.cos + pos * p.cos_ss, p.sin + pos * p.sin_ss);
-      rotate_unit<MODE, T, D>(a, b8, u, p.rotary, t, y);
-    };
-    auto store = [&](int e, const float (&y)[16], float inv) {
-      const int r = e / UPR, u = e % UPR;
-      int ca, cb;
-      unit_chunks<MODE>(u, p.rotary, ca, cb);
-      uint8_t* row = base + (r0 + r) * dst_ss;
-      put_codes(row, ca, y, inv);
-      put_codes(row, cb, y + 8, inv);
-    };
-    float held[kAppendHold][16];
-    float amax = 0.f;   // (fmaxf passes over NaN)
+  const int64_t page = L / c.page_size + nth;
+  if (page * c.page_size >= end) return;
+  const int pid = c.table[b * c.table_sb + page];
+  if (pid < 0 || pid >= c.num_pages) return;
+  const int64_t first = page * c.page_size;
+  const int r0 = (int)(max((int64_t)L, first) - first);                // first new row of the page
+  const int rows = (int)(min(end, first + c.page_size) - first) - r0;
+  if (rows <= 0) return;
+  const int64_t i0 = first + r0 - L;                                   // its token
+  const int total = rows * UPR;
+  uint8_t* base = cache + pid * dst_sp;
+  float* sp = scales + pid * scale_sp;
+  const float old = r0 > 0 ? *sp : 0.f;   // filled from its first row on: the old scale is another sequence's
+  auto load = [&](int e, float (&y)[16]) {
+    const int r = e / UPR, u = e % UPR;
+    int ca, cb;
+    unit_chunks<MODE>(u, p.rotary, ca, cb);
+    const T* row = src + (i0 + r) * src_ss;
+    const int64_t pos = first + r0 + r;
+    const vec8<T> a = ld8(row + ca * 8), b8 = ld8(row + cb * 8);
+    const Angles t = unit_angles<MODE>(u, p.rotary, p.cos + pos * p.cos_ss, p.sin + pos * p.sin_ss);
+    rotate_unit<MODE, T, D>(a, b8, u, p.rotary, t, y);
+  };
+  auto store = [&](int e, const float (&y)[16], float inv) {
+    const int r = e / UPR, u = e % UPR;
+    int ca, cb;
+    unit_chunks<MODE>(u, p.rotary, ca, cb);
+    uint8_t* row = base + (r0 + r) * dst_ss;
+    put_codes(row, ca, y, inv);
+    put_codes(row, cb, y + 8, inv);
+  };
+  float held[kAppendHold][16];
+  float amax = 0.f;   // (fmaxf passes over NaN)
 #pragma unroll
-    for (int q = 0; q < kAppendHold; ++q) {
-      const int e = tid + q * nt;
-      if (e < total) {
-        load(e, held[q]);
+  for (int q = 0; q < kAppendHold; ++q) {
+    const int e = tid + q * nt;
+    if (e < total) {
+      load(e, held[q]);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(held[q][j]));
-      }
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(held[q][j]));
     }
-    for (int e = tid + kAppendHold * nt; e < total; e += nt) {
+  }
+  for (int e = tid + kAppendHold * nt; e < total; e += nt) {
+    float y[16];
+    load(e, y);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(y[j]));
+  }
+  auto of_all = [&](float x) {   // the largest of the workgroup's threads
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+    __syncthreads();   // what wave_max held has been read
+    if ((tid & 63) == 0) wave_max[tid >> 6] = x;
+    __syncthreads();
+    for (int w = 0; w < (nt + 63) / 64; ++w) x = fmaxf(x, wave_max[w]);
+    return x;
+  };
+  amax = of_all(amax);
+  const bool infinite = amax == INFINITY;
+  if (infinite) {   // once more, of the finite ones
+    amax = 0.f;
+    for (int e = tid; e < total; e += nt) {
       float y[16];
       load(e, y);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(y[j]));
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(y[j]) < INFINITY ? fabsf(y[j]) : 0.f);
     }
-    auto of_all = [&](float x) {   // the largest of the workgroup's threads
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-      __syncthreads();   // what wave_max held has been read
-      if ((tid & 63) == 0) wave_max[tid >> 6] = x;
-      __syncthreads();
-      for (int w = 0; w < (nt + 63) / 64; ++w) x = fmaxf(x, wave_max[w]);
-      return x;
-    };
     amax = of_all(amax);
-    const bool infinite = amax == INFINITY;
-    if (infinite) {   // once more, of the finite ones
-      amax = 0.f;
-      for (int e = tid; e < total; e += nt) {
-        float y[16];
-        load(e, y);
+  }
+  const float scale = fmaxf(old, page_scale(amax));   // (an old NaN counts as none)
+  const float inv = 1.f / scale;
+  if (tid == 0) *sp = scale;
+  if (r0 > 0 && scale > old) {   // the rows before the new ones, in the new units
+    const float ratio = old * inv;
+    for (int e = tid; e < r0 * UPR; e += nt) {
+      u32x4* at = reinterpret_cast<u32x4*>(base + (int64_t)(e / UPR) * dst_ss + (e % UPR) * 16);
+      u32x4 x = *at;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(y[j]) < INFINITY ? fabsf(y[j]) : 0.f);
+      for (int j = 0; j < 4; ++j) {
+        float y[4];
+        e4m3_unpack4(x[j], y);
+        x[j] = e4m3_pack4(y[0] * ratio, y[1] * ratio, y[2] * ratio, y[3] * ratio);
       }
-      amax = of_all(amax);
+      *at = x;
     }
-    const float scale = fmaxf(old, page_scale(amax));   // (an old NaN counts as none)
-    const float inv = 1.f / scale;
-    if (tid == 0) *sp = scale;
-    if (r0 > 0 && scale > old) {   // the rows before the new ones, in the new units
-      const float ratio = old * inv;
-      for (int e = tid; e < r0 * UPR; e += nt) {
-        u32x4* at = reinterpret_cast<u32x4*>(base + (int64_t)(e / UPR) * dst_ss + (e % UPR) * 16);
-        u32x4 x = *at;
+  }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float y[4];
-          e4m3_unpack4(x[j], y);
-          x[j] = e4m3_pack4(y[0] * ratio, y[1] * ratio, y[2] * ratio, y[3] * ratio);
-        }
-        *at = x;
-      }
+  for (int q = 0; q < kAppendHold; ++q) {
+    const int e = tid + q * nt;
+    if (e < total) {
+      if (infinite) scale_saturated(held[q], inv);
+      store(e, held[q], infinite ? 1.f : inv);
     }
-#pragma unroll
-    for (int q = 0; q < kAppendHold; ++q) {
-      const int e = tid + q * nt;
-      if (e < total) {
-        if (infinite) scale_saturated(held[q], inv);
-        store(e, held[q], infinite ? 1.f : inv);
-      }
-    }
-    for (int e = tid + kAppendHold * nt; e < total; e += nt) {
-      float y[16];
-      load(e, y);
-      if (infinite) scale_saturated(y, inv);
-      store(e, y, infinite ? 1.f : inv);
-    }
+  }
+  for (int e = tid + kAppendHold * nt; e < total; e += nt) {
+    float y[16];
+    load(e, y);
+    if (infinite) scale_saturated(y, inv);
+    store(e, y, infinite ? 1.f : inv);
   }
 }
 
-// Blocks below `page_blocks` write codes, the others rows.
+// Page `item` of all that packed tokens touch, sequence by sequence: the sequence and which of
+// its pages; false past the last.
+__device__ __forceinline__ bool touched_page(const PagedCache& c, int64_t item, int& b, int& nth) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < c.B; base += 64 * kBlocks) {
+    uint32_t n[kBlocks], sum[kBlocks];
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+      const int s = base + 64 * k + lane;
+      n[k] = 0;
+      if (s < c.B) {
+        int off, len;
+        seg_bounds(c.cu, s, c.total, off, len);
+        const int L = max(c.seqlens[s], 0), end = (int)min((int64_t)L + len, (int64_t)c.capacity);
+        if (end > L) n[k] = (uint32_t)(end - 1) / (uint32_t)c.page_size - (uint32_t)L / (uint32_t)c.page_size + 1;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+      if (base + 64 * k >= c.B) return false;
+      sum[k] = (uint32_t)lanes_scan((int)n[k]);
+      const uint32_t all = lane_of(sum[k], 63);
+      if (item < all) {
+        uint32_t r = (uint32_t)item;
+        b = base + 64 * k + lane_of_item(n[k], sum[k], r);
+        nth = (int)r;
+        return nth >= 0;   // (less only if offsets are not monotone and the pages' sum passed 32 bits)
+      }
+      item -= all;
+    }
+  }
+  return false;
+}
+
+// Blocks below `page_blocks` write codes, the others rows.  A workgroup takes one page, of packed
+// tokens more if they touch more than the host counted on.  (A workgroup per sequence and page of
+// the longest one's: 255 tokens and a prompt of 8192, 916 us; by touched pages 77.)
 template <class T, bool FP8, int D>
 __global__ void __launch_bounds__(kAppendThreads)
 paged_append_kernel(PagedAppendParams p, int page_blocks) {
@@ -340,18 +402,22 @@ paged_append_kernel(PagedAppendParams p, int page_blocks) {
     int rest = blockIdx.x / c.Hkv;
     const bool is_v = rest & 1;
     rest >>= 1;
-    const int b = rest / p.pages_per_seq, first = rest % p.pages_per_seq;
-    if (is_v) {
-      append_codes<kNoRotation, T, D>(p, b, h, first, (const T*)p.v + (c.cu ? 0 : b * p.v_sb) + h * p.v_sh, p.v_ss,
-                                      (uint8_t*)c.v + h * c.v_sh, c.v_sp, c.v_ss, c.v_scale + h * c.vs_sh, c.vs_sp, wave_max);
-      return;
-    }
-    const T* k = (const T*)p.k + (c.cu ? 0 : b * p.k_sb) + h * p.k_sh;
-    uint8_t* to = (uint8_t*)c.k + h * c.k_sh;
-    float* sc = c.k_scale + h * c.ks_sh;
-    if (!p.rotary) append_codes<kNoRotation, T, D>(p, b, h, first, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
-    else if (p.interleaved) append_codes<kInterleaved, T, D>(p, b, h, first, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
-    else append_codes<kHalves, T, D>(p, b, h, first, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
+    int64_t item = rest;
+    do {
+      int b = rest / p.pages_per_seq, nth = rest % p.pages_per_seq;
+      if (c.cu && !touched_page(c, item, b, nth)) return;
+      if (is_v) {
+        append_codes<kNoRotation, T, D>(p, b, h, nth, (const T*)p.v + (c.cu ? 0 : b * p.v_sb) + h * p.v_sh, p.v_ss,
+                                        (uint8_t*)c.v + h * c.v_sh, c.v_sp, c.v_ss, c.v_scale + h * c.vs_sh, c.vs_sp, wave_max);
+        continue;
+      }
+      const T* k = (const T*)p.k + (c.cu ? 0 : b * p.k_sb) + h * p.k_sh;
+      uint8_t* to = (uint8_t*)c.k + h * c.k_sh;
+      float* sc = c.k_scale + h * c.ks_sh;
+      if (!p.rotary) append_codes<kNoRotation, T, D>(p, b, h, nth, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
+      else if (p.interleaved) append_codes<kInterleaved, T, D>(p, b, h, nth, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
+      else append_codes<kHalves, T, D>(p, b, h, nth, k, p.k_ss, to, c.k_sp, c.k_ss, sc, c.ks_sp, wave_max);
+    } while (c.cu && (item += p.page_items, true));
   }
 }
 
@@ -364,7 +430,7 @@ static hipError_t launch_append_t(const PagedAppendParams& pin, hipStream_t st) 
   const int rows = c.n < c.page_size ? c.n : c.page_size;
   int nt = FP8 ? (rows * (D / 16) + 64 * kAppendHold - 1) / (64 * kAppendHold) * 64 : 256;
   nt = nt > kAppendThreads ? kAppendThreads : nt < 64 ? 64 : nt;
-  const int64_t pages = FP8 ? (int64_t)c.B * p.pages_per_seq * 2 * c.Hkv : 0;
+  const int64_t pages = FP8 ? (int64_t)p.page_items * 2 * c.Hkv : 0;
   const int64_t items = (int64_t)c.total * p.row_groups * (D / 16);
   const int64_t blocks = pages + (items + nt - 1) / nt;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
@@ -465,7 +531,6 @@ __device__ __forceinline__ u32x2 lds_tr8(const uint8_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(p)));
 }
 
-__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
 __device__ __forceinline__ float lane_of(float x, int lane) { return __uint_as_float(lane_of(__float_as_uint(x), lane)); }
 
 // Slice layout of V in LDS: 16 rows in 16-byte chunks, chunk index XOR-swizzled by the row so
@@ -518,23 +583,10 @@ struct Runs {
 
 __device__ __forceinline__ int cache_rows(const PagedCache& c, int b) { return min(max(c.seqlens[b], 0), c.capacity); }
 
-// Inclusive sum over the wave's lanes (row shifts, then the rows' last lanes broadcast)
-__device__ __forceinline__ int lanes_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31
-  return x;
-}
-
-// Units of the sequences, by blocks of 64, one sequence per lane; four blocks are read at once, so
-// that large batches cost one round trip to memory in 256.  The first unit of a sequence has no
+// Units of the sequences, by blocks of 64, one sequence per lane.  The first unit of a sequence has no
 // rows: it stands for what starting and ending one costs (page table, scales, first rows, merge),
 // so that runs that cross into the next sequence get fewer rows and all end together (24
 // sequences of 77 to 4099 rows in 21 runs per head: 37.3 -> 35.3 us).
-constexpr int kBlocks = 4;
 struct UnitBlocks {
   int unit[kBlocks], sum[kBlocks];   // a lane's units, and the inclusive sums within its block
   __device__ UnitBlocks(const PagedCache& c, int base, int unit_rows, int lane) {
@@ -1046,6 +1098,56 @@ __device__ __attribute__((noinline)) void column_again(const PagedAttnParams& p,
   else if (p.lse) p.lse[row] = lse2 * kLn2;
 }
 
+// Item `item` of the tiles of tc columns of packed tokens: sequence and tile; false past the last.
+// In the order of the tiles' numbers, the last first (they see the most rows), by 256 sequences.
+// The tiles numbered x and more are the sum over the sequences of max(tiles - x, 0): the item's
+// number is the largest x of which that sum passes it.  (A workgroup for every sequence and tile
+// of the longest one's: 255 tokens and a prompt of 8192, 3065 us; by the tiles there are 948.)
+__device__ __forceinline__ bool tile_of_item(const PagedCache& c, int tc, int64_t item, int& b, int& ct) {
+  const int lane = threadIdx.x & 63, G = c.Hq / c.Hkv;
+  for (int base = 0; base < c.B; base += 64 * kBlocks) {
+    int n[kBlocks], most = 0;
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+      const int s = base + 64 * k + lane;
+      int off, len = 0;
+      if (s < c.B) seg_bounds(c.cu, s, c.total, off, len);
+      n[k] = cdiv(len * G, tc);
+      most = max(most, n[k]);
+    }
+    auto from = [&](int x) {
+      int sum = 0;
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) sum += max(n[k] - x, 0);
+      return lane_of((uint32_t)lanes_scan(sum), 63);
+    };
+    const uint32_t all = from(0);
+    if (item >= all) {
+      item -= all;
+      continue;
+    }
+    int bit = 0, x = 0;
+    while (bit < 30 && __ballot(most >> bit)) ++bit;
+    while (--bit >= 0)
+      if (from(x | 1 << bit) > item) x |= 1 << bit;
+    uint32_t r = (uint32_t)item - from(x + 1);
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+      auto more = __ballot(n[k] > x);
+      const uint32_t cnt = __builtin_popcountll(more);
+      if (r < cnt) {
+        for (; r; --r) more &= more - 1;
+        b = base + 64 * k + __builtin_ctzll(more);
+        ct = x;
+        return true;
+      }
+      r -= cnt;
+    }
+    return false;   // (offsets that are not monotone, whose tiles' sum passed 32 bits)
+  }
+  return false;
+}
+
 template <class T, bool FP8, int D, int RS>
 __global__ void __launch_bounds__(256, D > 128 ? 1 : 2)
 paged_tile_kernel(PagedAttnParams p) {
@@ -1078,21 +1180,23 @@ paged_tile_kernel(PagedAttnParams p) {
   int rest = blockIdx.x;
   const int hkv = rest % c.Hkv;
   rest /= c.Hkv;
-  const int b = rest % c.B;
-  rest /= c.B;
   const int split = rest % p.splits;
-  int off, len;
-  token_range(c, b, off, len);
-  const int L = cache_rows(c, b), ncols = len * G;
+  rest /= p.splits;
   const char* const kbase = (const char*)c.k + hkv * c.k_sh * CB;
   const char* const vbase = (const char*)c.v + hkv * c.v_sh * CB;
   const float* const kscale = FP8 ? c.k_scale + hkv * c.ks_sh : nullptr;
   const float* const vscale = FP8 ? c.v_scale + hkv * c.vs_sh : nullptr;
   const uint32_t k_page = (uint32_t)(c.k_sp * CB >> 4), v_page = (uint32_t)(c.v_sp * CB >> 4);   // 16-byte units
   const int step_pages = TR / c.page_size, step_rows = TR - step_pages * c.page_size;
-  // column tiles, those that see the most rows first; past the stated longest sequence each
-  // workgroup takes further ones
-  for (int ct = p.tile_cols - 1 - rest / p.splits; ct * TC < ncols; ct += p.tile_cols) {
+  // column tiles, those that see the most rows first (packed tokens: more than one only where
+  // sequences overlap or pass the stated longest)
+  int64_t item = rest;
+  do {
+    int b = rest % c.B, ct = p.tile_cols - 1 - rest / c.B;
+    if (c.cu && !tile_of_item(c, TC, item, b, ct)) return;
+    int off, len;
+    token_range(c, b, off, len);
+    const int L = cache_rows(c, b), ncols = len * G;
     const int col_last = min(ncols, (ct + 1) * TC) - 1;
     const int k_hi = max(p.causal ? L - len + col_last / G + 1 : L, 0);
     const int tiles = cdiv(k_hi, TR);
@@ -1381,7 +1485,7 @@ paged_tile_kernel(PagedAttnParams p) {
     }
     for (; marked; marked &= marked - 1)
       column_again<T, FP8, D>(args_again<PagedAttnParams>(), b, hkv, ct * TC + wc * 32 + __builtin_ctzll(marked), split, t0 * TR, t1 * TR);
-  }
+  } while (c.cu && (item += p.items, true));
 }
 
 // Merge the pieces' partial outputs of (token, query head) rows, W waves to a row and four waves
@@ -1544,9 +1648,9 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64
     // head dim 256) once, at most 16 and of four tiles at least.
     r.row_split = cols <= kTileCols / 2 && d <= 128 ? 2 : 1;
     const int64_t tile_cols = kTileCols / r.row_split, tiles = (cols + tile_cols - 1) / tile_cols;
-    r.tile_cols = (int)tiles;
     // column tiles of packed tokens: at most one that is not full in each sequence
     const int64_t all = std::max<int64_t>(std::min(B * tiles, total * (Hq / Hkv) / tile_cols + B), 1);
+    r.tile_cols = (int)tiles, r.items = all;
     const int64_t blocks = Hkv * all, slots = (int64_t)ncu * (d > 128 ? 1 : 2);
     const int64_t longest = (capacity + 4 * tile_rows(d) - 1) / (4 * tile_rows(d));
     const int64_t n = std::min<int64_t>({(slots + blocks / 2) / blocks, 16, longest});
