@@ -1098,21 +1098,22 @@ __device__ __attribute__((noinline)) void column_again(const PagedAttnParams& p,
   else if (p.lse) p.lse[row] = lse2 * kLn2;
 }
 
-// Item `item` of the tiles of tc columns of packed tokens: sequence and tile; false past the last.
+// Item `item` of the tiles of tc columns of packed tokens: sequence (its first token, tokens
+// and rows too: all of its loads go out at once) and tile; false past the last.
 // In the order of the tiles' numbers, the last first (they see the most rows), by 256 sequences.
 // The tiles numbered x and more are the sum over the sequences of max(tiles - x, 0): the item's
 // number is the largest x of which that sum passes it.  (A workgroup for every sequence and tile
 // of the longest one's: 255 tokens and a prompt of 8192, 3065 us; by the tiles there are 948.)
-__device__ __forceinline__ bool tile_of_item(const PagedCache& c, int tc, int64_t item, int& b, int& ct) {
+__device__ __forceinline__ bool tile_of_item(const PagedCache& c, int tc, int64_t item, int& b, int& ct, int& off, int& len, int& L) {
   const int lane = threadIdx.x & 63, G = c.Hq / c.Hkv;
   for (int base = 0; base < c.B; base += 64 * kBlocks) {
-    int n[kBlocks], most = 0;
+    int n[kBlocks], first[kBlocks], tokens[kBlocks], rows[kBlocks], most = 0;
 #pragma unroll
     for (int k = 0; k < kBlocks; ++k) {
       const int s = base + 64 * k + lane;
-      int off, len = 0;
-      if (s < c.B) seg_bounds(c.cu, s, c.total, off, len);
-      n[k] = cdiv(len * G, tc);
+      first[k] = tokens[k] = rows[k] = 0;
+      if (s < c.B) seg_bounds(c.cu, s, c.total, first[k], tokens[k]), rows[k] = cache_rows(c, s);
+      n[k] = cdiv(tokens[k] * G, tc);
       most = max(most, n[k]);
     }
     auto from = [&](int x) {
@@ -1137,8 +1138,10 @@ __device__ __forceinline__ bool tile_of_item(const PagedCache& c, int tc, int64_
       const uint32_t cnt = __builtin_popcountll(more);
       if (r < cnt) {
         for (; r; --r) more &= more - 1;
-        b = base + 64 * k + __builtin_ctzll(more);
-        ct = x;
+        const int at = __builtin_ctzll(more);
+        b = base + 64 * k + at, ct = x;
+        off = (int)lane_of((uint32_t)first[k], at), len = (int)lane_of((uint32_t)tokens[k], at);
+        L = (int)lane_of((uint32_t)rows[k], at);
         return true;
       }
       r -= cnt;
@@ -1192,11 +1195,10 @@ paged_tile_kernel(PagedAttnParams p) {
   // sequences overlap or pass the stated longest)
   int64_t item = rest;
   do {
-    int b = rest % c.B, ct = p.tile_cols - 1 - rest / c.B;
-    if (c.cu && !tile_of_item(c, TC, item, b, ct)) return;
-    int off, len;
-    token_range(c, b, off, len);
-    const int L = cache_rows(c, b), ncols = len * G;
+    int b = rest % c.B, ct = p.tile_cols - 1 - rest / c.B, off = 0, len = c.n, L;
+    if (!c.cu) L = cache_rows(c, b);
+    else if (!tile_of_item(c, TC, item, b, ct, off, len, L)) return;
+    const int ncols = len * G;
     const int col_last = min(ncols, (ct + 1) * TC) - 1;
     const int k_hi = max(p.causal ? L - len + col_last / G + 1 : L, 0);
     const int tiles = cdiv(k_hi, TR);
