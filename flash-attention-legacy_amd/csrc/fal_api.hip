@@ -972,8 +972,9 @@ int paged_append_impl(const fal_paged_cache* cache, const void* k, const void* v
 
 // Rows of partial outputs in the workspace
 size_t paged_partials(const PagedPlan& plan, const fal_paged_cache& c) {
-  if (plan.splits) return plan.splits > 1 ? (size_t)c.total_tokens * c.heads_q * plan.splits : 0;
-  return plan.direct ? 0 : (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols;
+  const size_t tiled = plan.splits > 1 ? (size_t)c.total_tokens * c.heads_q * plan.splits : 0;
+  const size_t runs = plan.parts && !plan.direct ? (size_t)(plan.parts + c.batch) * c.heads_kv * plan.cols : 0;
+  return std::max(tiled, runs);   // (where both kernels run, one after the other)
 }
 
 PagedPlan plan_of(const fal_paged_cache& c) {
@@ -1004,6 +1005,7 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
   p.parts = plan.parts, p.unit_rows = plan.unit_rows, p.wave_heads = plan.wave_heads;
   p.nc = plan.nc, p.col_tiles = plan.col_tiles, p.cols = plan.cols, p.direct = plan.direct;
   p.splits = plan.splits, p.tile_cols = plan.tile_cols, p.row_split = plan.row_split, p.items = plan.items;
+  p.c.most = plan.most;
   const size_t rows = paged_partials(plan, c);
   p.part_o = static_cast<float*>(workspace);
   p.part_m = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(rows * c.head_dim * sizeof(float)));
@@ -1014,8 +1016,9 @@ int paged_attn_impl(const fal_paged_cache* cache, const void* q, void* o, float*
     if (plan.items > (0x7fffffff - 64) / per) return fail(FAL_ERR_INVALID, "problem too large for one launch");
     p.tile_blocks = (int)(plan.items * per);
     p.rest_blocks = c.cu_seqlens ? 16 : 0;
-  } else if ((int64_t)plan.parts * c.heads_kv * plan.col_tiles > 0x7fffffff ||
-             c.batch * ((c.max_pages * c.page_size + plan.unit_rows - 1) / plan.unit_rows + 1) / plan.parts >= 0x7fffffff)
+  }
+  if (plan.parts && ((int64_t)plan.parts * c.heads_kv * plan.col_tiles > 0x7fffffff ||
+                     c.batch * ((c.max_pages * c.page_size + plan.unit_rows - 1) / plan.unit_rows + 1) / plan.parts >= 0x7fffffff))
     return fail(FAL_ERR_INVALID, "problem too large for one launch");
   return launch_status(launch_paged_attn(p, (int)c.head_dim, static_cast<hipStream_t>(stream)), "fal_paged_attn");
 }

@@ -155,6 +155,7 @@ struct PagedCache {
   int B, n, Hq, Hkv;
   int total;          // tokens in all (B * n without cu)
   int num_pages, page_size, capacity;   // capacity = max_pages * page_size
+  int most;           // attention, packed: 0, or the tokens up to which a sequence is the split kernel's
   int fp8;
   int bf16;           // element type of the 16-bit tensors: 0 fp16, 1 bf16
 };
@@ -195,13 +196,14 @@ struct PagedAttnParams {
   // outside every sequence
   int64_t items;
   int splits, tile_cols, row_split, tile_blocks, rest_blocks;   // row_split: waves that share a column's rows
-  float* part_o;      // [parts + B, Hkv, cols, d], or [total, Hq, splits, d]
+  float* part_o;      // [parts + B, Hkv, cols, d], or [total, Hq, splits, d], or one after the other
   float* part_m;      // the same without d: log2-domain LSE
 };
 struct PagedPlan {
   int parts, unit_rows, wave_heads, nc, col_tiles, cols, direct;
   int splits, tile_cols, row_split;
   int64_t items;
+  int most;
 };
 
 hipError_t launch_fwd(const FwdParams& p, int d, int causal, dim3 grid, hipStream_t st);

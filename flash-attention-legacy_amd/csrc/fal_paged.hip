@@ -583,6 +583,14 @@ struct Runs {
 
 __device__ __forceinline__ int cache_rows(const PagedCache& c, int b) { return min(max(c.seqlens[b], 0), c.capacity); }
 
+// Packed sequences that both kernels share: the split kernel takes those of up to c.most tokens,
+// the tile kernel the others.  Rows of sequence b for the split kernel:
+__device__ __forceinline__ int split_rows(const PagedCache& c, int b) {
+  int off, len = 0;
+  if (c.most) seg_bounds(c.cu, b, c.total, off, len);
+  return c.most && len > c.most ? 0 : cache_rows(c, b);
+}
+
 // Units of the sequences, by blocks of 64, one sequence per lane.  The first unit of a sequence has no
 // rows: it stands for what starting and ending one costs (page table, scales, first rows, merge),
 // so that runs that cross into the next sequence get fewer rows and all end together (24
@@ -593,7 +601,7 @@ struct UnitBlocks {
 #pragma unroll
     for (int k = 0; k < kBlocks; ++k) {
       const int b = base + 64 * k + lane;
-      const int rows = b < c.B ? cache_rows(c, b) : 0;
+      const int rows = b < c.B ? split_rows(c, b) : 0;
       unit[k] = rows > 0 ? cdiv(rows, unit_rows) + 1 : 0;
     }
 #pragma unroll
@@ -764,7 +772,7 @@ paged_split_kernel(PagedAttnParams p) {
   const int vc0 = FP8 ? VS::swz(vr, kk >> 2) : ((l16 >> 1) & 1) ^ VS::swz(vr, 0);
 
   for (; left > 0 && b < c.B; ++b, local = 0) {
-    const int L = cache_rows(c, b);
+    const int L = split_rows(c, b);
     const int take = min(left, (L > 0 ? cdiv(L, p.unit_rows) + 1 : 0) - local);
     left = p.direct ? 0 : left - take;
     const int row0 = max(local - 1, 0) * p.unit_rows, row1 = min(L, (local + take - 1) * p.unit_rows);
@@ -1113,7 +1121,7 @@ __device__ __forceinline__ bool tile_of_item(const PagedCache& c, int tc, int64_
       const int s = base + 64 * k + lane;
       first[k] = tokens[k] = rows[k] = 0;
       if (s < c.B) seg_bounds(c.cu, s, c.total, first[k], tokens[k]), rows[k] = cache_rows(c, s);
-      n[k] = cdiv(tokens[k] * G, tc);
+      n[k] = tokens[k] > c.most ? cdiv(tokens[k] * G, tc) : 0;
       most = max(most, n[k]);
     }
     auto from = [&](int x) {
@@ -1502,14 +1510,21 @@ paged_combine_kernel(PagedAttnParams p) {
   __shared__ float m_s[4], l_s[4], o_s[4][D];
   const PagedCache& c = p.c;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x * (4 / W) + (W == 4 ? 0 : wave);
-  if (row >= (int64_t)c.total * c.Hq) return;
+  int64_t row = (int64_t)blockIdx.x * (4 / W) + (W == 4 ? 0 : wave);
+  if (row >= (c.most ? (int64_t)c.B * c.most : c.total) * c.Hq) return;
   const int w = W == 4 ? wave : 0;
-  const int h = (int)(row % c.Hq), t = (int)(row / c.Hq);
-  int b = 0, i = 0, ns = 0;
-  const bool in = token_place(c, t, b, i);
-  int off = 0, len = 1;
-  if (in) token_range(c, b, off, len);
+  const int h = (int)(row % c.Hq);
+  int t = (int)(row / c.Hq), b = 0, i = 0, ns = 0, off = 0, len = 1;
+  bool in;
+  if (c.most) {   // the sequences of few tokens, each with places for c.most
+    b = t / c.most, i = t - b * c.most;
+    token_range(c, b, off, len);
+    if (i >= len || len > c.most) return;
+    in = true, t = off + i, row = (int64_t)t * c.Hq + h;
+  } else {
+    in = token_place(c, t, b, i);
+    if (in) token_range(c, b, off, len);
+  }
   const bool alone = in && (i >= c.n || (c.n == 1 && len > 1));   // past the stated longest sequence
   const int G = c.Hq / c.Hkv;
   int64_t base = 0, step = (int64_t)c.Hkv * p.cols;
@@ -1619,6 +1634,11 @@ paged_merge_kernel(PagedAttnParams p) {
   const int t = (int)(row / c.Hq), h = (int)(row % c.Hq);
   int b, n;
   const bool in = token_place(c, t, b, n);
+  if (in && c.most) {   // the split kernel's
+    int off, len;
+    token_range(c, b, off, len);
+    if (len <= c.most) return;
+  }
   const float* pm = p.part_m + row * p.splits;
   const f32x4* po = reinterpret_cast<const f32x4*>(p.part_o + row * p.splits * D + d);
   float M = -INFINITY, sum = 0.f;
@@ -1644,20 +1664,29 @@ constexpr int kDirectRows = 2048;   // longest caches that one workgroup takes w
 PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64_t Hkv, int64_t capacity, int d, bool fp8,
                      bool packed, int ncu) {
   PagedPlan r{};
-  const int64_t cols = (seqlen > 0 ? seqlen : 1) * (Hq / Hkv);
+  const int64_t G = Hq / Hkv;
+  int64_t cols = (seqlen > 0 ? seqlen : 1) * G;
   if (cols > kSplitCols) {
+    // Sequences of few tokens (one tile of 16 columns, or one token) among packed longer ones go
+    // to the split kernel, as a prompt's chunk and running sequences make up one step: where all
+    // but the longest have that few on average (255 tokens behind 2000 rows and 2048 of a prompt
+    // 403 -> 296 us; 63 behind 8000 364 -> 250).  Elsewhere the second pair of launches finds little to do.
+    const int64_t few = std::max<int64_t>(16 / G, 1), others = std::max<int64_t>(total - seqlen, 0);
+    if (packed && B > 1 && few * G <= kSplitCols && others <= (B - 1) * few && B * few * Hq < (1 << 24)) r.most = (int)few;
     // The tile kernel.  Splits: as many as fill the workgroup slots (two per compute unit, one at
     // head dim 256) once, at most 16 and of four tiles at least.
     r.row_split = cols <= kTileCols / 2 && d <= 128 ? 2 : 1;
     const int64_t tile_cols = kTileCols / r.row_split, tiles = (cols + tile_cols - 1) / tile_cols;
     // column tiles of packed tokens: at most one that is not full in each sequence
-    const int64_t all = std::max<int64_t>(std::min(B * tiles, total * (Hq / Hkv) / tile_cols + B), 1);
+    const int64_t part = r.most ? std::min(B, 1 + others / (few + 1)) : B;
+    const int64_t all = std::max<int64_t>(std::min(B * tiles, total * G / tile_cols + part), 1);
     r.tile_cols = (int)tiles, r.items = all;
     const int64_t blocks = Hkv * all, slots = (int64_t)ncu * (d > 128 ? 1 : 2);
     const int64_t longest = (capacity + 4 * tile_rows(d) - 1) / (4 * tile_rows(d));
     const int64_t n = std::min<int64_t>({(slots + blocks / 2) / blocks, 16, longest});
     r.splits = (int)std::max<int64_t>(n, 1);
-    return r;
+    if (!r.most) return r;
+    cols = few * G;
   }
   const int waves = paged_waves(d, fp8);
   r.nc = cols <= 16 || d > 128 ? 1 : 2;   // (head dim 256: two tiles would not fit the registers)
@@ -1667,7 +1696,7 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64
   // short ones (1000 rows: 12.9 us, in runs 13.5; 512 workgroups of up to 1500 rows: 41 us, in
   // runs 36).
   // (Of one token: results that are not finite under a mask are the second kernel's.)
-  r.direct = capacity <= kDirectRows && !packed && seqlen == 1 && B * Hkv * r.col_tiles <= ncu;
+  r.direct = !r.most && capacity <= kDirectRows && !packed && seqlen == 1 && B * Hkv * r.col_tiles <= ncu;
   // KV heads of a workgroup, by the rows that its run has at most (measured on 32/8 heads of 128,
   // 8 bits, with 1 / 2 / 4 heads): 4096 x 4 rows 18.7 / 18.5 / 19.8 us, 16 x 8000 43.2 / 41.3 /
   // 42.6, 64 x 2500 54.5 / 45.5 / 46.6, 32 x 32768 206 / 186 / 178.
@@ -1683,16 +1712,19 @@ PagedPlan paged_plan(int64_t B, int64_t seqlen, int64_t total, int64_t Hq, int64
 }
 
 template <class T, bool FP8, int D>
-static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
+static hipError_t launch_attn_t(PagedAttnParams p, hipStream_t st) {
   if (p.splits) {
     const dim3 tiles((unsigned)(p.tile_blocks + (p.splits > 1 ? 0 : p.rest_blocks)));
     if (D > 128 || p.row_split == 1) hipLaunchKernelGGL((paged_tile_kernel<T, FP8, D, 1>), tiles, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((paged_tile_kernel<T, FP8, (D > 128 ? 128 : D), 2>), tiles, dim3(256), 0, st, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    const int64_t threads = (int64_t)p.c.total * p.c.Hq * (D / 4);
-    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, p);
-    return hipGetLastError();
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && p.splits > 1) {
+      const int64_t threads = (int64_t)p.c.total * p.c.Hq * (D / 4);
+      hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, p);
+      e = hipGetLastError();
+    }
+    if (e != hipSuccess || !p.c.most) return e;
+    p.c.n = p.c.most;   // and the sequences of few tokens
   }
   const dim3 grid((unsigned)(p.parts * (p.c.Hkv / p.wave_heads) * p.col_tiles)), block(paged_waves(D, FP8) * 64);
   constexpr int D2 = D > 128 ? 128 : D;   // (two tiles: up to head dim 128)
@@ -1706,7 +1738,7 @@ static hipError_t launch_attn_t(const PagedAttnParams& p, hipStream_t st) {
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.direct) return e;
-  const int64_t rows = (int64_t)p.c.total * p.c.Hq;
+  const int64_t rows = (p.c.most ? (int64_t)p.c.B * p.c.most : p.c.total) * p.c.Hq;
   if (p.parts / p.c.B < 8)   // (pieces of a sequence, about)
     hipLaunchKernelGGL((paged_combine_kernel<T, FP8, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
   else

@@ -656,6 +656,35 @@ def test_prompt_and_single_tokens_in_one_batch(cache):
     check_attend(pool, q, after, new, got)
 
 
+FEW_AND_MANY = [
+    # d, hkv, hq, dtype, lens (with the new rows), new
+    (128, 2, 8, torch.bfloat16, [700, 5, 333, 90, 40, 3], [4, 5, 200, 1, 0, 3]),
+    (256, 1, 2, torch.float16, [30, 150, 300, 1, 64, 77], [8, 9, 150, 1, 2, 1]),
+    (64, 4, 4, torch.float16, [16, 290, 90, 33, 0], [16, 17, 90, 2, 1]),
+    (96, 1, 20, torch.bfloat16, [1, 20, 100, 260, 65, 7], [1, 0, 30, 1, 2, 0]),
+    (128, 2, 8, torch.float16, [600, 500, 40, 30, 5], [1, 12, 2, 0, 5]),
+    (32, 8, 32, torch.float16, [100, 2100, 900], [1, 2048, 2]),
+]
+
+
+@pytest.mark.parametrize("cache", ["fp8", "same"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", FEW_AND_MANY, ids=lambda c: f"d{c[0]}h{c[1]}-{c[2]}n{max(c[5])}")
+def test_attend_few_and_many_tokens_packed(case, causal, cache):
+    """Sequences around the number of tokens up to which another kernel takes them, rows outside
+    every sequence, and the longest stated exactly, too long and too short."""
+    d, hkv, hq, dtype, lens, new = case
+    pool = Pool(len(lens), -(-max(lens) // 16) + 1, 16, hkv, d, cache, dtype, seed=d + hq)
+    front, back = 3, 5
+    cu = (torch.tensor(starts_of(new), dtype=torch.int32) + front).cuda()
+    q = randn((front + sum(new) + back, hq, d), 1, dtype, 2.0)
+    for longest in (max(new), q.shape[0], 2, max(new) // 2):
+        o, lse = pool.attend(q, lens, causal=causal, return_softmax_lse=True, cu_seqlens_q=cu, max_seqlen_q=longest)
+        for x in (slice(0, front), slice(-back, None)):
+            assert bool((o[x] == 0).all()) and bool(torch.isneginf(lse[x]).all())
+        check_attend(pool, q[front:-back], lens, new, (o[front:-back], lse[front:-back]), causal)
+
+
 @pytest.mark.parametrize("cache", ["fp8", "same"])
 def test_rejected_tokens_are_written_over(cache):
     """Speculative decoding: five tokens proposed, two kept, the next five start behind those."""
