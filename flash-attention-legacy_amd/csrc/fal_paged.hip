@@ -1111,8 +1111,13 @@ __device__ __attribute__((noinline)) void column_again(const PagedAttnParams& p,
 // In the order of the tiles' numbers, the last first (they see the most rows), by 256 sequences.
 // The tiles numbered x and more are the sum over the sequences of max(tiles - x, 0): the item's
 // number is the largest x of which that sum passes it.  (A workgroup for every sequence and tile
-// of the longest one's: 255 tokens and a prompt of 8192, 3065 us; by the tiles there are 948.)
-__device__ __forceinline__ bool tile_of_item(const PagedCache& c, int tc, int64_t item, int& b, int& ct, int& off, int& len, int& L) {
+// of the longest one's: 255 tokens and a prompt of 8192, 3065 us; by the tiles there are 948.
+// Not inlined: inlined it cost the loop behind it (chunk of 1024 tokens 184 -> 191 us, so 186).)
+struct TileItem {
+  int b, ct, off, len, rows;   // b < 0: none
+};
+__device__ __attribute__((noinline)) TileItem tile_of_item(const PagedAttnParams& p, int tc, int64_t item) {
+  const PagedCache& c = p.c;
   const int lane = threadIdx.x & 63, G = c.Hq / c.Hkv;
   for (int base = 0; base < c.B; base += 64 * kBlocks) {
     int n[kBlocks], first[kBlocks], tokens[kBlocks], rows[kBlocks], most = 0;
@@ -1147,16 +1152,14 @@ __device__ __forceinline__ bool tile_of_item(const PagedCache& c, int tc, int64_
       if (r < cnt) {
         for (; r; --r) more &= more - 1;
         const int at = __builtin_ctzll(more);
-        b = base + 64 * k + at, ct = x;
-        off = (int)lane_of((uint32_t)first[k], at), len = (int)lane_of((uint32_t)tokens[k], at);
-        L = (int)lane_of((uint32_t)rows[k], at);
-        return true;
+        return {base + 64 * k + at, x, (int)lane_of((uint32_t)first[k], at), (int)lane_of((uint32_t)tokens[k], at),
+                (int)lane_of((uint32_t)rows[k], at)};
       }
       r -= cnt;
     }
-    return false;   // (offsets that are not monotone, whose tiles' sum passed 32 bits)
+    break;   // (offsets that are not monotone, whose tiles' sum passed 32 bits)
   }
-  return false;
+  return {-1, 0, 0, 0, 0};
 }
 
 template <class T, bool FP8, int D, int RS>
@@ -1203,9 +1206,13 @@ paged_tile_kernel(PagedAttnParams p) {
   // sequences overlap or pass the stated longest)
   int64_t item = rest;
   do {
-    int b = rest % c.B, ct = p.tile_cols - 1 - rest / c.B, off = 0, len = c.n, L;
-    if (!c.cu) L = cache_rows(c, b);
-    else if (!tile_of_item(c, TC, item, b, ct, off, len, L)) return;
+    TileItem it;
+    if (c.cu) it = tile_of_item(args_again<PagedAttnParams>(), TC, item);
+    else it = {rest % c.B, p.tile_cols - 1 - rest / c.B, 0, c.n, cache_rows(c, rest % c.B)};
+    const int b = __builtin_amdgcn_readfirstlane(it.b), ct = __builtin_amdgcn_readfirstlane(it.ct);
+    const int off = __builtin_amdgcn_readfirstlane(it.off), len = __builtin_amdgcn_readfirstlane(it.len);
+    const int L = __builtin_amdgcn_readfirstlane(it.rows);
+    if (b < 0) return;
     const int ncols = len * G;
     const int col_last = min(ncols, (ct + 1) * TC) - 1;
     const int k_hi = max(p.causal ? L - len + col_last / G + 1 : L, 0);
