@@ -686,6 +686,37 @@ def test_attend_few_and_many_tokens_packed(case, causal, cache):
 
 
 @pytest.mark.parametrize("cache", ["fp8", "same"])
+@pytest.mark.parametrize("most", [1, 24])
+def test_hundreds_of_packed_sequences(most, cache):
+    """More sequences than are searched at once, of one token or of up to 24, long ones among them."""
+    g = torch.Generator().manual_seed(most)
+    n = 600
+    new = torch.randint(0, most + 1, (n,), generator=g).tolist()
+    new[0], new[299], new[599] = 70, 33, 90
+    lens = torch.randint(0, 30, (n,), generator=g).tolist()
+    pool = Pool(n, 8, 16, 1, 32, cache, seed=23)
+    k, v, q = (randn((sum(new), h, 32), i) for i, h in enumerate((1, 1, 2)))
+    starts = starts_of(new)
+    tensor = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    before = snapshot(pool)
+    pool.append(k, v, lens, cu_seqlens=tensor(starts), max_seqlen=max(new))
+    got = snapshot(pool)
+    for name, t in before.items():
+        getattr(pool, name).copy_(t)
+    table = pool.table
+    for a in range(0, n, 200):   # the same in three calls
+        t0, t1 = starts[a], starts[a + 200]
+        pool.table = table[a:a + 200]
+        pool.append(k[t0:t1], v[t0:t1], lens[a:a + 200], cu_seqlens=tensor([t - t0 for t in starts[a:a + 201]]), max_seqlen=90)
+    pool.table = table
+    for name, t in got.items():
+        assert same(getattr(pool, name), t), name
+    after = [x + y for x, y in zip(lens, new)]
+    res = pool.attend(q, after, return_softmax_lse=True, cu_seqlens_q=tensor(starts), max_seqlen_q=max(new))
+    check_attend(pool, q, after, new, res)
+
+
+@pytest.mark.parametrize("cache", ["fp8", "same"])
 def test_rejected_tokens_are_written_over(cache):
     """Speculative decoding: five tokens proposed, two kept, the next five start behind those."""
     pool = Pool(2, 3, 32, 2, 64, cache, seed=17)
